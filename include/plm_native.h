@@ -254,6 +254,93 @@ typedef struct plm_add_rmsnorm_desc {
   int32_t corr_ld;
 } plm_add_rmsnorm_desc;
 
+/* ---- paged caches of several sequences (plm_cache_append, plm_cache_attention) ----
+ * No counterpart in the reference, whose round decodes one request from 16-bit pages: an append that rotates queries and
+ * keys on the way into the pages, pages of 16-bit or 8-bit numbers, and attention over them for any number of
+ * sequences, with or without a sliding window. */
+enum plm_cache_kind {
+  PLM_CACHE_MODEL = 0, /* pages in the model dtype */
+  PLM_CACHE_E4M3 = 1   /* pages of e4m3 codes; a value is its code times the scale of its block of tokens and head */
+};
+
+typedef struct plm_paged_cache {
+  int32_t kind;         /* enum plm_cache_kind */
+  void* k;              /* [num_pages][num_kv_heads][page_size][head_dim], 16-byte aligned */
+  void* v;
+  float* k_scale;       /* PLM_CACHE_E4M3: [num_pages][num_kv_heads][page_size / scale_block], finite, above 0 */
+  float* v_scale;
+  int32_t scale_block;  /* PLM_CACHE_E4M3: tokens that share a scale; a power of two, at most page_size and 64 */
+  int32_t num_pages;
+  int32_t page_size;    /* a power of two, at most 4096 */
+  int32_t num_kv_heads;
+  int32_t head_dim;     /* 64 or 128 */
+} plm_paged_cache;
+
+/* The sequences of a call. Sequence s has the rows row_start[s] .. row_start[s + 1] - 1 of the call's row buffers, at
+ * the logical cache indices context[s], context[s] + 1, ...; the cache holds its first context[s] tokens (and, for
+ * attention, the rows' own too). Everything the device arrays say may change between replays of a captured call; what
+ * contradicts the host's bounds (rows, max_rows, max_pages), or a negative length, is recorded as an index out of range,
+ * and that sequence is skipped. A sequence without rows is left out. */
+typedef struct plm_sequences {
+  int32_t n_seqs;              /* 1..65535 */
+  int32_t max_rows;            /* rows of the longest sequence, at most */
+  int64_t max_keys;            /* context + rows of the longest sequence, about: attention divides long ones by it */
+  const int32_t* row_start;    /* [n_seqs + 1] */
+  const int64_t* context;      /* [n_seqs] */
+  const int32_t* block_tables; /* [n_seqs][table_stride]: logical page -> physical page */
+  int64_t table_stride;
+  int32_t max_pages;           /* entries of a block table, at most table_stride */
+} plm_sequences;
+
+/* Rotates the rows' queries and keys (neox halves: out[i] = x[i] cos[i] - x[i + d/2] sin[i], out[i + d/2] =
+ * x[i + d/2] cos[i] + x[i] sin[i], in fp32) and writes the keys and values into the pages. Every value is rounded
+ * once, to the model dtype or to e4m3. In e4m3 pages the scale of a block and head is 2^e, e the smallest integer with
+ * max|x| <= 448 * 2^e over the call's finite values of that block, at least -100. A block that holds earlier tokens of
+ * its sequence keeps the larger of the new and the old scale, and those tokens' codes are brought to it; tokens behind
+ * the appended ones in the block are no longer valid. Infinities become +-448 times the scale, NaN stays NaN. Rows that no
+ * sequence holds, and pages and blocks that no row falls into, are left as they were. No two sequences of a call may
+ * append into one page. */
+typedef struct plm_cache_append_desc {
+  int32_t dtype;           /* enum plm_dtype: q, k, v, q_out, cos_sin and 16-bit pages */
+  int32_t rows;            /* rows of the buffers */
+  const void* q;           /* nullable: [rows][num_heads][head_dim], rows q_stride elements apart */
+  const void* k;           /* [rows][num_kv_heads][head_dim] */
+  const void* v;
+  int64_t q_stride, k_stride, v_stride; /* elements; multiples of 8 */
+  void* q_out;             /* with q: rows q_out_stride apart; may be q itself */
+  int64_t q_out_stride;
+  int32_t num_heads;
+  int32_t max_pos;         /* rows of cos_sin */
+  const void* cos_sin;     /* nullable (no rotation): [max_pos][head_dim], cos | sin halves */
+  const int32_t* positions; /* nullable (the logical index): [rows] */
+  plm_paged_cache cache;
+  plm_sequences seqs;
+} plm_cache_append_desc;
+
+/* Attention of the rows over their sequences' cached keys. With p = context + depth (causal: depth[j] = j) key kv is
+ * visible to row j of its sequence iff
+ *     kv <= p  and  (window == 0  or  kv < sinks  or  kv > pos - window),
+ *     or  own_start[j] <= kv - context <= j   (depth and own_start given: the round mask of plm_attention),
+ * where pos is p, plus j - own_start[j] inside an own block. A row that sees no key gives zeros. Keys that no row sees
+ * need no page: a window's caller may have given the pages behind it away. Rows that no sequence holds are left as
+ * they were. */
+typedef struct plm_cache_attention_desc {
+  int32_t dtype;
+  int32_t rows;             /* rows of q and out */
+  const void* q;            /* [rows][num_heads][head_dim], rows q_stride elements apart */
+  int64_t q_stride;
+  void* out;                /* [rows][num_heads][head_dim], rows out_stride elements apart */
+  int64_t out_stride;
+  int32_t num_heads;        /* a multiple of num_kv_heads */
+  float scale;              /* of the scores; 0: 1 / sqrt(head_dim) */
+  int32_t window;           /* 0: unbounded */
+  int32_t sinks;            /* first tokens that stay visible behind the window */
+  const int32_t* depth;     /* nullable: [rows] relative to the row's context */
+  const int32_t* own_start; /* nullable, with depth: [rows] */
+  plm_paged_cache cache;
+  plm_sequences seqs;
+} plm_cache_attention_desc;
+
 /* ---- round engine (one handle = one request stream on one GPU, batch 1) ---- */
 typedef struct plm_handle plm_handle;
 
@@ -397,6 +484,9 @@ int plm_attention(plm_ctx* ctx, const plm_attention_desc* desc, void* stream);
 int plm_kv_append(plm_ctx* ctx, const plm_kv_append_desc* desc, void* stream);
 int plm_add_rmsnorm(plm_ctx* ctx, const plm_add_rmsnorm_desc* desc, void* stream);
 int plm_commit(plm_ctx* ctx, const plm_commit_desc* desc, void* stream);
+/* Both use no memory of the context but its error word, so calls on several streams and captured graphs may overlap. */
+int plm_cache_append(plm_ctx* ctx, const plm_cache_append_desc* desc, void* stream);
+int plm_cache_attention(plm_ctx* ctx, const plm_cache_attention_desc* desc, void* stream);
 
 /* ---- round engine ---- */
 int plm_create(const plm_model_desc* model, const plm_weight_ptrs* weights, const plm_round_desc* round,

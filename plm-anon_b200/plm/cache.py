@@ -1,0 +1,234 @@
+"""Paged caches of several sequences: rotating and appending keys and values, and attention over them.
+
+``PagedCache`` holds the pages, in the model dtype or as e4m3 codes with a scale for each block of tokens and head;
+``Sequences`` says which rows of a call belong to which sequence, how many tokens each has in the cache, and where its
+pages are. ``append`` and ``attention`` enqueue ``plm_cache_append`` and ``plm_cache_attention`` (include/plm_native.h
+has the definitions) on the current stream and never synchronise, so both can be captured into a CUDA graph; a replay
+reads the lengths and block tables anew from the tensors of its ``Sequences``.
+
+    cache = PagedCache.allocate(num_pages, kv_heads, 64, 128, dtype="e4m3", scale_block=32)
+    seqs = Sequences(row_start, context, block_tables, max_rows=1, max_keys=8192)
+    q = append(ctx, cache, seqs, k, v, q=q, cos_sin=decoder.cos_sin)
+    out = attention(ctx, cache, seqs, q, window=4096, sinks=4)
+
+What contradicts the host's bounds on the device (a row range, a page, a position) is skipped and recorded:
+``Context.check`` raises for it.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import native
+from .native import NativeError
+
+MAX_SCALE_BLOCK = 64
+_MODEL_DTYPES = {torch.bfloat16: native.PLM_BF16, torch.float16: native.PLM_F16}
+
+
+def _same_device(what: str, device: torch.device, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise NativeError(f"{what}: {name} is on {t.device}, not on {device}")
+
+
+class PagedCache:
+    """Pages of keys and values, [num_pages, kv_heads, page_size, head_dim] each: bfloat16 or float16, or
+    float8_e4m3fn with ``k_scale`` and ``v_scale`` [num_pages, kv_heads, page_size / scale_block] float32."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None = None,
+                 v_scale: torch.Tensor | None = None) -> None:
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
+            raise NativeError("PagedCache: k and v are [num_pages, kv_heads, page_size, head_dim] of one shape and dtype")
+        if not (k.is_contiguous() and v.is_contiguous()):
+            raise NativeError("PagedCache: k and v must be contiguous")
+        pages, kv_heads, page, head_dim = k.shape
+        e4m3 = k.dtype == torch.float8_e4m3fn
+        if not e4m3 and k.dtype not in _MODEL_DTYPES:
+            raise NativeError(f"PagedCache: pages of {k.dtype} (bfloat16, float16 or float8_e4m3fn)")
+        if e4m3 != (k_scale is not None) or e4m3 != (v_scale is not None):
+            raise NativeError("PagedCache: float8_e4m3fn pages have k_scale and v_scale, 16-bit pages have none")
+        block = 0
+        if e4m3:
+            for name, s in (("k_scale", k_scale), ("v_scale", v_scale)):
+                if s.dtype != torch.float32 or s.dim() != 3 or not s.is_contiguous() or s.shape != k_scale.shape or \
+                        s.shape[:2] != k.shape[:2] or s.shape[2] < 1 or page % s.shape[2]:
+                    raise NativeError(f"PagedCache: {name} is contiguous float32 [num_pages, kv_heads, page_size / "
+                                      "scale_block]")
+            block = page // k_scale.shape[2]
+        _same_device("PagedCache", k.device, v=v, k_scale=k_scale, v_scale=v_scale)
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = pages, kv_heads, page, head_dim
+        self.scale_block = block
+        self.dtype, self.device = k.dtype, k.device
+        self.desc = native.PagedCacheDesc(
+            kind=native.CACHE_E4M3 if e4m3 else native.CACHE_MODEL, k=k.data_ptr(), v=v.data_ptr(),
+            k_scale=native.ptr(k_scale), v_scale=native.ptr(v_scale), scale_block=block, num_pages=pages,
+            page_size=page, num_kv_heads=kv_heads, head_dim=head_dim)
+
+    @classmethod
+    def allocate(cls, num_pages: int, num_kv_heads: int, page_size: int, head_dim: int, *,
+                 dtype: torch.dtype | str = torch.bfloat16, scale_block: int = 16,
+                 device: torch.device | str = "cuda") -> "PagedCache":
+        """Zeroed pages. ``dtype`` is bfloat16, float16, or "e4m3" for codes with a scale per ``scale_block`` tokens
+        (a power of two, at most the page size and 64)."""
+        shape = (num_pages, num_kv_heads, page_size, head_dim)
+        if dtype not in ("e4m3", torch.float8_e4m3fn):
+            return cls(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device))
+        if scale_block < 1 or scale_block > min(page_size, MAX_SCALE_BLOCK) or page_size % scale_block:
+            raise NativeError(f"PagedCache: {scale_block} tokens to a scale with pages of {page_size}")
+        scales = (num_pages, num_kv_heads, page_size // scale_block)
+        codes = [torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn) for _ in range(2)]
+        return cls(*codes, torch.ones(scales, device=device), torch.ones(scales, device=device))
+
+
+class Sequences:
+    """The sequences of a call, on the device: ``row_start`` int32 [n + 1], the first row of each (and the end of the
+    last); ``context`` int64 [n], the tokens each has in the cache before its rows; ``block_tables`` int32
+    [n, max_pages], logical to physical page. ``max_rows`` bounds the rows of one sequence, ``max_keys`` its context and
+    rows together (how attention divides long caches goes by it; the default is what a block table can hold)."""
+
+    def __init__(self, row_start: torch.Tensor, context: torch.Tensor, block_tables: torch.Tensor, *, max_rows: int,
+                 max_keys: int = 0) -> None:
+        n = context.numel()
+        if row_start.dtype != torch.int32 or row_start.dim() != 1 or row_start.numel() != n + 1 or \
+                not row_start.is_contiguous():
+            raise NativeError("Sequences: row_start is contiguous int32 [n + 1]")
+        if context.dtype != torch.int64 or context.dim() != 1 or n < 1 or not context.is_contiguous():
+            raise NativeError("Sequences: context is contiguous int64 [n]")
+        if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.shape[0] != n or \
+                block_tables.shape[1] < 1 or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1):
+            raise NativeError("Sequences: block_tables is int32 [n, max_pages] with contiguous rows")
+        if max_rows < 1 or max_keys < 0:
+            raise NativeError(f"Sequences: at most {max_rows} rows and {max_keys} keys to a sequence")
+        _same_device("Sequences", row_start.device, context=context, block_tables=block_tables)
+        self.row_start, self.context, self.block_tables = row_start, context, block_tables
+        self.count, self.max_rows, self.max_keys, self.device = n, max_rows, max_keys, row_start.device
+        pages = block_tables.shape[1]
+        self.desc = native.SequencesDesc(
+            n_seqs=n, max_rows=max_rows, max_keys=max_keys, row_start=row_start.data_ptr(), context=context.data_ptr(),
+            block_tables=block_tables.data_ptr(), table_stride=block_tables.stride(0) if n > 1 else pages,
+            max_pages=pages)
+
+
+def _heads(what: str, name: str, t: torch.Tensor, rows: int, heads: int | None, head_dim: int, dtype) -> int:
+    """Checks [rows, heads, head_dim] with heads side by side in a row; returns the row stride in elements."""
+    shape = t.shape
+    if len(shape) != 3 or shape[0] != rows or shape[2] != head_dim or (heads is not None and shape[1] != heads):
+        raise NativeError(f"{what}: {name} is {list(shape)}, not [{rows}, {heads or 'heads'}, {head_dim}]")
+    if t.dtype != dtype:
+        raise NativeError(f"{what}: {name} is {t.dtype}, not {dtype}")
+    stride = t.stride()
+    if stride[2] != 1 or (shape[1] > 1 and stride[1] != head_dim):
+        raise NativeError(f"{what}: the heads of a row of {name} must be contiguous")
+    return stride[0] if rows > 1 else shape[1] * head_dim
+
+
+def _common(what: str, ctx, cache: PagedCache, seqs: Sequences, rows: int, dtype) -> int:
+    code = _MODEL_DTYPES.get(dtype)
+    if code is None:
+        raise NativeError(f"{what}: rows of {dtype} (bfloat16 or float16)")
+    if cache.desc.kind == native.CACHE_MODEL and cache.dtype != dtype:
+        raise NativeError(f"{what}: rows of {dtype} and pages of {cache.dtype}")
+    if rows < 1:
+        raise NativeError(f"{what}: no rows")
+    return code
+
+
+def _device(what: str, ctx, cache: PagedCache, seqs: Sequences, **tensors) -> torch.device:
+    device = torch.device("cuda", ctx.device)
+    _same_device(what, device, cache=cache, sequences=seqs, **tensors)
+    return device
+
+
+def _table(what: str, name: str, t: torch.Tensor | None, rows: int) -> int | None:
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != rows or (rows > 1 and t.stride(0) != 1):
+        raise NativeError(f"{what}: {name} is contiguous int32 [{rows}]")
+    return t.data_ptr()
+
+
+def _output(like: torch.Tensor, stream) -> torch.Tensor:
+    """An output tensor owned by the stream that writes it."""
+    if stream is None:
+        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+    with torch.cuda.stream(stream):
+        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+
+
+def append(ctx: native.Context, cache: PagedCache, seqs: Sequences, k: torch.Tensor, v: torch.Tensor, *,
+           q: torch.Tensor | None = None, q_out: torch.Tensor | None = None, cos_sin: torch.Tensor | None = None,
+           positions: torch.Tensor | None = None, stream=None) -> torch.Tensor | None:
+    """Rotates the rows' ``q`` and ``k`` by ``cos_sin`` ([max_pos, head_dim]: cos | sin, as ``rope_cache`` makes it; None:
+    no rotation) at ``positions`` (int32 [rows]; None: the logical indices) and writes ``k`` and ``v`` into the pages.
+
+    ``q`` [rows, heads, head_dim], ``k`` and ``v`` [rows, kv_heads, head_dim] may be slices of one projection's rows.
+    Returns the rotated queries: ``q_out`` (``q`` itself is allowed), or a new tensor whose rows no sequence holds are
+    not written. e4m3 pages: the call sets the scales of the blocks it begins and raises those it continues, bringing
+    the tokens before its own to the new scale; tokens behind the appended ones in a block are no longer valid."""
+    what = "cache.append"
+    rows, hd = k.shape[0], cache.head_dim
+    dtype = k.dtype
+    code = _common(what, ctx, cache, seqs, rows, dtype)
+    desc = native.CacheAppendDesc(dtype=code, rows=rows, cache=cache.desc, seqs=seqs.desc)
+    desc.k_stride = _heads(what, "k", k, rows, cache.num_kv_heads, hd, dtype)
+    desc.v_stride = _heads(what, "v", v, rows, cache.num_kv_heads, hd, dtype)
+    if q is not None:
+        desc.q_stride = _heads(what, "q", q, rows, None, hd, dtype)
+        desc.num_heads = q.shape[1]
+        if q_out is not None:
+            desc.q_out_stride = _heads(what, "q_out", q_out, rows, q.shape[1], hd, dtype)
+    elif q_out is not None:
+        raise NativeError(f"{what}: q_out without q")
+    if cos_sin is not None:
+        if cos_sin.dtype != dtype or cos_sin.dim() != 2 or cos_sin.shape[1] != hd or not cos_sin.is_contiguous():
+            raise NativeError(f"{what}: cos_sin is contiguous {dtype} [max_pos, {hd}]")
+        desc.cos_sin, desc.max_pos = cos_sin.data_ptr(), cos_sin.shape[0]
+    desc.positions = _table(what, "positions", positions, rows)
+    device = _device(what, ctx, cache, seqs, k=k, v=v, q=q, q_out=q_out, cos_sin=cos_sin, positions=positions)
+    if q is not None:
+        if q_out is None:
+            q_out = _output(q, stream)
+            desc.q_out_stride = q.shape[1] * hd
+        desc.q, desc.q_out = q.data_ptr(), q_out.data_ptr()
+    desc.k, desc.v = k.data_ptr(), v.data_ptr()
+    on = (stream if stream is not None else torch.cuda.current_stream(device)).cuda_stream
+    native.check(native.library().plm_cache_append(ctx.handle, ctypes.byref(desc), on), "plm_cache_append")
+    return q_out
+
+
+def attention(ctx: native.Context, cache: PagedCache, seqs: Sequences, q: torch.Tensor, *,
+              out: torch.Tensor | None = None, scale: float | None = None, window: int = 0, sinks: int = 0,
+              depth: torch.Tensor | None = None, own_start: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """Attention of ``q`` [rows, heads, head_dim] over the sequences' cached keys, the rows' own among them (append
+    first): causal, or under the round mask with ``depth`` and ``own_start`` (int32 [rows], as ``round_layout`` gives
+    them). With ``window`` a row sees its own position and the ``window - 1`` before it, and the first ``sinks`` tokens.
+    ``scale`` defaults to 1 / sqrt(head_dim). Returns ``out``, or a new tensor; rows that no sequence holds are not
+    written, and a row that sees no key gets zeros."""
+    what = "cache.attention"
+    rows, hd = q.shape[0], cache.head_dim
+    dtype = q.dtype
+    code = _common(what, ctx, cache, seqs, rows, dtype)
+    q_stride = _heads(what, "q", q, rows, None, hd, dtype)
+    heads = q.shape[1]
+    if heads % cache.num_kv_heads:
+        raise NativeError(f"{what}: {heads} heads over {cache.num_kv_heads} kv heads")
+    out_stride = _heads(what, "out", out, rows, heads, hd, dtype) if out is not None else heads * hd
+    if scale is not None and not 0.0 < scale < float("inf"):
+        raise NativeError(f"{what}: scale {scale}")
+    if (depth is None) != (own_start is None):
+        raise NativeError(f"{what}: depth and own_start go together")
+    depth_ptr, own_ptr = _table(what, "depth", depth, rows), _table(what, "own_start", own_start, rows)
+    device = _device(what, ctx, cache, seqs, q=q, out=out, depth=depth, own_start=own_start)
+    if out is None:
+        out = _output(q, stream)
+    desc = native.CacheAttentionDesc(
+        dtype=code, rows=rows, q=q.data_ptr(), q_stride=q_stride, out=out.data_ptr(), out_stride=out_stride,
+        num_heads=heads, scale=scale or 0.0, window=window, sinks=sinks, depth=depth_ptr, own_start=own_ptr,
+        cache=cache.desc, seqs=seqs.desc)
+    on = (stream if stream is not None else torch.cuda.current_stream(device)).cuda_stream
+    native.check(native.library().plm_cache_attention(ctx.handle, ctypes.byref(desc), on), "plm_cache_attention")
+    return out

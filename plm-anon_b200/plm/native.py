@@ -99,6 +99,34 @@ class CommitDesc(ctypes.Structure):
                 ("commit", c_void_p)]
 
 
+CACHE_MODEL, CACHE_E4M3 = 0, 1
+
+
+class PagedCacheDesc(ctypes.Structure):
+    _fields_ = [("kind", c_int32), ("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p),
+                ("scale_block", c_int32), ("num_pages", c_int32), ("page_size", c_int32), ("num_kv_heads", c_int32),
+                ("head_dim", c_int32)]
+
+
+class SequencesDesc(ctypes.Structure):
+    _fields_ = [("n_seqs", c_int32), ("max_rows", c_int32), ("max_keys", c_int64), ("row_start", c_void_p),
+                ("context", c_void_p), ("block_tables", c_void_p), ("table_stride", c_int64), ("max_pages", c_int32)]
+
+
+class CacheAppendDesc(ctypes.Structure):
+    _fields_ = [("dtype", c_int32), ("rows", c_int32), ("q", c_void_p), ("k", c_void_p), ("v", c_void_p),
+                ("q_stride", c_int64), ("k_stride", c_int64), ("v_stride", c_int64), ("q_out", c_void_p),
+                ("q_out_stride", c_int64), ("num_heads", c_int32), ("max_pos", c_int32), ("cos_sin", c_void_p),
+                ("positions", c_void_p), ("cache", PagedCacheDesc), ("seqs", SequencesDesc)]
+
+
+class CacheAttentionDesc(ctypes.Structure):
+    _fields_ = [("dtype", c_int32), ("rows", c_int32), ("q", c_void_p), ("q_stride", c_int64), ("out", c_void_p),
+                ("out_stride", c_int64), ("num_heads", c_int32), ("scale", ctypes.c_float), ("window", c_int32),
+                ("sinks", c_int32), ("depth", c_void_p), ("own_start", c_void_p), ("cache", PagedCacheDesc),
+                ("seqs", SequencesDesc)]
+
+
 class ModelDesc(ctypes.Structure):
     _fields_ = [("dtype", c_int32), ("num_layers", c_int32), ("hidden", c_int32), ("num_heads", c_int32),
                 ("num_kv_heads", c_int32), ("head_dim", c_int32), ("intermediate", c_int32), ("vocab", c_int32),
@@ -162,6 +190,8 @@ _SIGNATURES: dict[str, list] = {
     "plm_kv_append": [c_void_p, POINTER(KvAppendDesc), c_void_p],
     "plm_add_rmsnorm": [c_void_p, POINTER(AddRmsNormDesc), c_void_p],
     "plm_commit": [c_void_p, POINTER(CommitDesc), c_void_p],
+    "plm_cache_append": [c_void_p, POINTER(CacheAppendDesc), c_void_p],
+    "plm_cache_attention": [c_void_p, POINTER(CacheAttentionDesc), c_void_p],
     "plm_icdf_decode": [c_void_p, POINTER(IcdfDesc), c_void_p],
     "plm_block_schedule": [c_int32, c_int32, c_int32, c_int32, POINTER(c_int32), c_int32, POINTER(c_int32),
                            POINTER(c_int32)],
@@ -231,6 +261,9 @@ class Context:
         handle = c_void_p()
         check(library().plm_ctx_create(ctypes.byref(handle)), "plm_ctx_create")
         self.handle = handle
+        import torch
+
+        self.device = torch.cuda.current_device()  # the index of the device it is bound to
 
     def check(self) -> None:
         """Synchronise and raise if any kernel recorded a device error since the last check."""
@@ -290,6 +323,16 @@ def add_rmsnorm(ctx: Context, desc: AddRmsNormDesc, stream=None) -> None:
 def commit(ctx: Context, desc: CommitDesc, stream=None) -> None:
     """Enqueue plm_commit: the rows the device commit record names, from round scratch into the paged cache."""
     check(library().plm_commit(ctx.handle, ctypes.byref(desc), stream_handle(stream)), "plm_commit")
+
+
+def cache_append(ctx: Context, desc: CacheAppendDesc, stream=None) -> None:
+    """Enqueue plm_cache_append (``plm.cache.append`` takes tensors and checks them)."""
+    check(library().plm_cache_append(ctx.handle, ctypes.byref(desc), stream_handle(stream)), "plm_cache_append")
+
+
+def cache_attention(ctx: Context, desc: CacheAttentionDesc, stream=None) -> None:
+    """Enqueue plm_cache_attention (``plm.cache.attention`` takes tensors and checks them)."""
+    check(library().plm_cache_attention(ctx.handle, ctypes.byref(desc), stream_handle(stream)), "plm_cache_attention")
 
 
 def block_schedule(num_sms: int, hidden: int, intermediate: int, q_size: int) -> list[list[int]]:
