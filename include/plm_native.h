@@ -321,9 +321,9 @@ typedef struct plm_cache_append_desc {
  * visible to row j of its sequence iff
  *     kv <= p  and  (window == 0  or  kv < sinks  or  kv > pos - window),
  *     or  own_start[j] <= kv - context <= j   (depth and own_start given: the round mask of plm_attention),
- * where pos is p, plus j - own_start[j] inside an own block. A row that sees no key gives zeros. Keys that no row sees
- * need no page: a window's caller may have given the pages behind it away. Rows that no sequence holds are left as
- * they were. */
+ * where pos is p, plus j - own_start[j] inside an own block. A row that sees no key gives zeros. Behind the sinks, keys
+ * below the first one that a row sees need no page: a window's caller may have given those pages away. Rows that no
+ * sequence holds are left as they were. */
 typedef struct plm_cache_attention_desc {
   int32_t dtype;
   int32_t rows;             /* rows of q and out */

@@ -1,0 +1,23 @@
+// Argument block of attention over a paged cache, shared by its kernels (cache_attention.cu, cache_prefill.cu).
+#pragma once
+
+#include "cache.h"
+
+namespace plm {
+
+struct CacheAttnArgs {
+  CachePages c;
+  CacheSeqs s;
+  const void* q;
+  int64_t q_stride;
+  void* out;
+  int64_t out_stride;
+  int heads, group;  // group: query heads of a kv head
+  float scale_log2;  // of the scores, in units of log2
+  int window, sinks;
+  const int32_t *depth, *own_start;
+  int splits;        // CTAs of a cluster that share a sequence's keys
+  int* err;
+};
+
+}  // namespace plm
