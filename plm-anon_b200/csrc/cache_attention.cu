@@ -7,10 +7,10 @@
 //     S^T[16 keys, rows] = K Q^T,      O^T[d, rows] += V^T P^T,
 // so 8 rows fill an instruction and a K or V element is brought into its fragment once for all rows. A product's inner
 // index may be permuted if both operands are, and an output's index if the store undoes it: thread (gq, tq) =
-// (lane / 4, lane % 4) takes the d/4 neighbouring elements [tq d/4, ...) of keys gq and gq + 8 as its part of K, and
-// the d/8 neighbouring elements [gq d/8, ...) of keys 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9 as its part of V. Both are
-// vectors in global memory, whole lines across the warp, so nothing is staged: the fragments of the next chunk are
-// loaded into the registers that the current one's have left. P^T changes sides through movmatrix.
+// (lane / 4, lane % 4) takes a quarter of the elements of keys gq and gq + 8 as its part of K, and an eighth of the
+// elements of keys 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9 as its part of V, both in whole vectors of shared memory.
+// P^T changes sides through movmatrix. Every warp has a ring of its own that 16-byte asynchronous copies keep full, so
+// the warps of a CTA meet only at the end, where their partial results are joined, and those of a cluster's CTAs.
 //
 // The softmax is online in base 2 with a lazy maximum: a row's m is raised (and O, l rescaled) only when a score passes
 // it by more than 2^8, so most chunks take one vote and no cross-lane maximum; weights stay below 2^8.
@@ -34,12 +34,13 @@
 namespace plm {
 namespace {
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kChunk = 16;          // keys
 constexpr int kMaxSplits = 8;       // CTAs of a portable cluster
 constexpr int kUnreachable = 1 << 30;
 constexpr float kLazy = 8.f;        // log2 of how far a weight may pass 1
+constexpr int kStages = 3;          // chunks of a warp's ring
 
 template <typename M>
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -73,18 +74,64 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return uint32_t(*reinterpret_cast<const uint16_t*>(&l)) | (uint32_t(*reinterpret_cast<const uint16_t*>(&h)) << 16);
 }
 
-// N neighbouring words, read once: past L1.
-template <int N>
-__device__ __forceinline__ void load_words(uint32_t (&r)[N], const uint8_t* p) {
-  if constexpr (N == 2) {
-    asm volatile("ld.global.nc.L1::no_allocate.v2.b32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "l"(p));
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; i += 4)
-      asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];"
-                   : "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3])
-                   : "l"(p + i * 4));
+// A chunk of 16 keys in shared memory: K rows, then V rows, then (e4m3) the 16 key scales and the 16 value scales. Rows
+// are vectors of 16 bytes, vector c of row `key` at c ^ swizzle(key), so that the eight threads of a load's phase (two
+// neighbouring gq, four tq) meet eight different groups of banks both in K (rows gq) and in V (rows 2 tq + const).
+template <int HD, bool E4M3>
+struct Chunk {
+  static constexpr int ES = E4M3 ? 1 : 2;
+  static constexpr int VECS = HD * ES / 16;  // vectors of a row
+  static constexpr int PLANE = kChunk * HD * ES;
+  static constexpr int BYTES = 2 * PLANE + (E4M3 ? 2 * kChunk * 4 : 0);
+  static constexpr int KW = HD / 4 * ES / 4;  // words a thread holds of a key
+  static constexpr int VW = HD / 8 * ES / 4;  // and of a value
+  static __device__ __forceinline__ int swizzle(int key) {
+    if (!E4M3) return ((key & 1) << 2) | ((key >> 1) & 3);
+    return VECS == 8 ? key & 7 : (key >> 1) & 3;
   }
+  static __device__ __forceinline__ int at(int key, int vec) { return key * (HD * ES) + ((vec ^ swizzle(key)) << 4); }
+  // Vector i of thread tq's part of a key, and the first of the 16 / ES elements in it.
+  static __device__ __forceinline__ int k_vec(int tq, int i) { return E4M3 ? tq * VECS / 4 + i : tq + 4 * i; }
+  // Thread gq's element 2 t of its part of a value.
+  static __device__ __forceinline__ int v_vec(int gq, int i) {
+    if (E4M3) return VECS == 8 ? gq : gq >> 1;
+    return (((gq & 1) << 2) | (gq >> 1)) + 8 * i;
+  }
+  static __device__ __forceinline__ int v_element(int gq, int t) {
+    return E4M3 ? gq * (HD / 8) + 2 * t : v_vec(gq, t / 4) * 8 + (t % 4) * 2;
+  }
+  static __device__ __forceinline__ void read_key(uint32_t (&r)[KW], const uint8_t* plane, int key, int tq) {
+#pragma unroll
+    for (int i = 0; i < KW / 4; ++i) {
+      const uint4 x = *reinterpret_cast<const uint4*>(plane + at(key, k_vec(tq, i)));
+      r[4 * i] = x.x;
+      r[4 * i + 1] = x.y;
+      r[4 * i + 2] = x.z;
+      r[4 * i + 3] = x.w;
+    }
+  }
+  static __device__ __forceinline__ void read_value(uint32_t (&r)[VW], const uint8_t* plane, int key, int gq) {
+    if constexpr (VW == 2) {
+      const uint2 x = *reinterpret_cast<const uint2*>(plane + at(key, v_vec(gq, 0)) + (gq & 1) * 8);
+      r[0] = x.x;
+      r[1] = x.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < VW / 4; ++i) {
+        const uint4 x = *reinterpret_cast<const uint4*>(plane + at(key, v_vec(gq, i)));
+        r[4 * i] = x.x;
+        r[4 * i + 1] = x.y;
+        r[4 * i + 2] = x.z;
+        r[4 * i + 3] = x.w;
+      }
+    }
+  }
+};
+
+// 4-byte asynchronous copy; `valid` false zero-fills.
+__device__ __forceinline__ void cp_async_4(void* smem_dst, const void* src, bool valid) {
+  const int size = valid ? 4 : 0;
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(smem_dst)), "l"(src), "r"(size) : "memory");
 }
 
 // What one packed row sees, as logical indices below 2^30: [first, last] and below `sinks`, and the own block.
@@ -111,15 +158,23 @@ __device__ __forceinline__ RowMask row_mask(const CacheAttnArgs& a, const SeqRan
   return m;
 }
 
+// The rings, and after the loop the warps' partial results in their place.
+template <int HD, bool E4M3, int NR>
+constexpr int decode_smem_bytes() {
+  constexpr int ring = kWarps * kStages * Chunk<HD, E4M3>::BYTES;
+  constexpr int partial = kWarps * 8 * NR * HD * 4;
+  return ring > partial ? ring : partial;
+}
+
 template <int HD, typename T, bool E4M3, int NR>
-__global__ void __launch_bounds__(kThreads) decode_attention_kernel(const CacheAttnArgs a) {
+__global__ void __launch_bounds__(kThreads, E4M3 && NR == 1 ? 2 : 1) decode_attention_kernel(const CacheAttnArgs a) {
   using M = typename std::conditional<E4M3, __half, T>::type;  // type of the products
-  constexpr int ES = E4M3 ? 1 : 2;
+  using C = Chunk<HD, E4M3>;
+  constexpr int ES = C::ES, KW = C::KW, VW = C::VW;
   constexpr int KS = HD / 16;           // steps of S over the head elements, and M tiles of O^T
-  constexpr int KW = HD / 4 * ES / 4;   // words a thread holds of a key
-  constexpr int VW = HD / 8 * ES / 4;   // and of a value
   constexpr int ROWS = 8 * NR;
-  __shared__ float po[kWarps][ROWS][HD];
+  extern __shared__ __align__(128) uint8_t smem[];
+  float(*po)[ROWS][HD] = reinterpret_cast<float(*)[ROWS][HD]>(smem);  // [kWarps], after the loop
   __shared__ float pm[kWarps][ROWS], pl[kWarps][ROWS];
   __shared__ float cm[ROWS], cl[ROWS];  // the CTA's own maxima and sums, for the cluster
 
@@ -161,7 +216,7 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const CacheA
   const int c_begin = int(int64_t(split) * chunks / a.splits), c_end = int(int64_t(split + 1) * chunks / a.splits);
   auto chunk_key = [&](int c) { return (c < sink_chunks ? c : lo / kChunk + c - sink_chunks) * kChunk; };
 
-  // ---- queries: B fragments of S^T, row 8 nr + gq, elements [tq d/4, ...)
+  // ---- queries: B fragments of S^T, row 8 nr + gq, the elements that thread tq has of a key
   uint32_t qf[NR][2 * KS];
   float q_scale[NR][2];  // of rows 8 nr + 2 tq and the next one
 #pragma unroll
@@ -172,10 +227,10 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const CacheA
     for (int w = 0; w < 2 * KS; ++w) qf[nr][w] = 0;
     if (live) {
       const T* src = static_cast<const T*>(a.q) + (r.start + i / a.group) * a.q_stride +
-                     (head * a.group + i % a.group) * HD + tq * (HD / 4);
+                     (head * a.group + i % a.group) * HD;
 #pragma unroll
       for (int w = 0; w < 2 * KS; w += 4) {
-        const uint4 v = *reinterpret_cast<const uint4*>(src + 2 * w);
+        const uint4 v = *reinterpret_cast<const uint4*>(src + (E4M3 ? tq * (HD / 4) + 2 * w : C::k_vec(tq, w / 4) * 8));
         qf[nr][w] = v.x;
         qf[nr][w + 1] = v.y;
         qf[nr][w + 2] = v.z;
@@ -227,40 +282,29 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const CacheA
     record_error(a.err, kErrBadIndex);
     return -1;
   };
-  auto load_k = [&](uint32_t (&k)[2][KW], int kv0, int pages) {
+  uint8_t* ring = smem + warp * kStages * C::BYTES;
+  // Chunk at kv0 into a stage of the warp's ring; what is not to be loaded becomes zeros.
+  auto issue = [&](int stage, int kv0, int pages) {
+    uint8_t* dst = ring + stage * C::BYTES;
+    constexpr int PER_PASS = 32 / C::VECS;  // rows
+    const int vec = lane % C::VECS;
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int key = gq + 8 * x;
+    for (int p = 0; p < kChunk / PER_PASS; ++p) {
+      const int key = p * PER_PASS + lane / C::VECS;
       const int page = __shfl_sync(0xffffffffu, pages, key);
-      if (page >= 0) {
-        const size_t at = (size_t(page) * a.c.kv_heads + head) * a.c.page_size + ((kv0 + key) & page_mask);
-        load_words<KW>(k[x], kp + (at * HD + tq * (HD / 4)) * ES);
-      } else {
-#pragma unroll
-        for (int w = 0; w < KW; ++w) k[x][w] = 0;
-      }
+      const bool valid = page >= 0;
+      const size_t row = (size_t(valid ? page : 0) * a.c.kv_heads + head) * a.c.page_size + ((kv0 + key) & page_mask);
+      const size_t from = row * (HD * ES) + vec * 16;
+      cp_async_16(dst + C::at(key, vec), kp + from, valid);
+      cp_async_16(dst + C::PLANE + C::at(key, vec), vp + from, valid);
     }
-  };
-  auto load_v = [&](uint32_t (&v)[4][VW], int kv0, int pages) {
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int key = 2 * tq + (x & 1) + (x >> 1) * 8;
-      const int page = __shfl_sync(0xffffffffu, pages, key);
-      if (page >= 0) {
-        const size_t at = (size_t(page) * a.c.kv_heads + head) * a.c.page_size + ((kv0 + key) & page_mask);
-        load_words<VW>(v[x], vp + (at * HD + gq * (HD / 8)) * ES);
-      } else {
-#pragma unroll
-        for (int w = 0; w < VW; ++w) v[x][w] = 0;
-      }
+    if constexpr (E4M3) {  // lanes 0..15 the keys' scales, lanes 16..31 the values'
+      const bool valid = pages >= 0;
+      const int slot = (kv0 + (lane & 15)) & page_mask;
+      const size_t block = (size_t(valid ? pages : 0) * a.c.kv_heads + head) * (a.c.page_size >> a.c.block_shift) +
+                           (slot >> a.c.block_shift);
+      cp_async_4(dst + 2 * C::PLANE + lane * 4, (lane < 16 ? a.c.k_scale : a.c.v_scale) + block, valid);
     }
-  };
-  // Scale of key (lane % 16): the keys' in lanes 0..15, the values' in 16..31.
-  auto load_scale = [&](int kv0, int pages) {
-    if (!E4M3 || pages < 0) return 1.f;
-    const int slot = (kv0 + (lane & 15)) & page_mask;
-    const size_t at = (size_t(pages) * a.c.kv_heads + head) * (a.c.page_size >> a.c.block_shift) + (slot >> a.c.block_shift);
-    return lane < 16 ? a.c.k_scale[at] : a.c.v_scale[at];
   };
 
   float o[KS][NR][4];
@@ -272,22 +316,31 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const CacheA
 #pragma unroll
     for (int t = 0; t < KS; ++t) o[t][nr][0] = o[t][nr][1] = o[t][nr][2] = o[t][nr][3] = 0.f;
   }
-  uint32_t k[2][KW], v[4][VW];
-  float scale = 1.f;
-  int c = c_begin + warp;
+  // One group of copies a chunk, empty ones included; kStages - 1 ahead of the chunk in work.
+  const int c_first = c_begin + warp;
   int pages = -1;
-  if (c < c_end) {
-    pages = pages_of(chunk_key(c));
-    load_k(k, chunk_key(c), pages);
-    load_v(v, chunk_key(c), pages);
-    scale = load_scale(chunk_key(c), pages);
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) {
+    const int c = c_first + i * kWarps;
+    if (c < c_end) issue(i, chunk_key(c), pages_of(chunk_key(c)));
+    cp_async_commit();
   }
-  int next_pages = c + kWarps < c_end ? pages_of(chunk_key(c + kWarps)) : -1;
+  if (c_first + (kStages - 1) * kWarps < c_end) pages = pages_of(chunk_key(c_first + (kStages - 1) * kWarps));
 
-  for (; c < c_end; c += kWarps) {
+  int stage = 0;
+  for (int c = c_first; c < c_end; c += kWarps) {
     const int kv0 = chunk_key(c);
-    const bool more = c + kWarps < c_end;
-    const int next_kv0 = more ? chunk_key(c + kWarps) : 0;
+    cp_async_wait<kStages - 2>();
+    __syncwarp();  // the chunk is there for every lane, and every lane is done with the one before it
+    const int c_next = c + (kStages - 1) * kWarps;
+    if (c_next < c_end) issue(stage == 0 ? kStages - 1 : stage - 1, chunk_key(c_next), pages);
+    cp_async_commit();
+    if (c_next + kWarps < c_end) pages = pages_of(chunk_key(c_next + kWarps));
+    const uint8_t* chunk = ring + stage * C::BYTES;
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+    uint32_t k[2][KW];
+    C::read_key(k[0], chunk, gq, tq);
+    C::read_key(k[1], chunk, gq + 8, tq);
     // ---- S^T = K Q^T, even and odd steps apart
     float s[NR][4], s_odd[NR][4];
 #pragma unroll
@@ -312,18 +365,17 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const CacheA
       for (int nr = 0; nr < NR; ++nr)
         mma_16816<M>(t & 1 ? s_odd[nr] : s[nr], f[0], f[1], f[2], f[3], qf[nr][2 * t], qf[nr][2 * t + 1]);
     }
-    const float now = scale;
-    if (more) {
-      load_k(k, next_kv0, next_pages);
-      scale = load_scale(next_kv0, next_pages);
-    }
+    uint32_t v[4][VW];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) C::read_value(v[x], chunk + C::PLANE, 2 * tq + (x & 1) + (x >> 1) * 8, gq);
     // ---- scores in units of log2, masks
     float log_v[2], inv_v[2], k_scale[2];
     if constexpr (E4M3) {
+      const float* scales = reinterpret_cast<const float*>(chunk + 2 * C::PLANE);
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        k_scale[x] = __shfl_sync(0xffffffffu, now, gq + 8 * x);
-        const float vs = fmaxf(__shfl_sync(0xffffffffu, now, 16 + gq + 8 * x), 7.888609052210118e-31f);  // 2^-100
+        k_scale[x] = scales[gq + 8 * x];
+        const float vs = fmaxf(scales[16 + gq + 8 * x], 7.888609052210118e-31f);  // 2^-100
         log_v[x] = log2f(vs);
         inv_v[x] = 1.f / vs;
       }
@@ -444,11 +496,11 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const CacheA
 #pragma unroll
       for (int nr = 0; nr < NR; ++nr) mma_16816<M>(o[t][nr], f[0], f[1], f[2], f[3], p[nr][0], p[nr][1]);
     }
-    if (more) load_v(v, next_kv0, next_pages);
-    next_pages = c + 2 * kWarps < c_end ? pages_of(chunk_key(c + 2 * kWarps)) : -1;
   }
+  cp_async_wait<0>();
+  __syncthreads();  // the rings make room for the partial results
 
-  // ---- the warps' partial results: row 8 nr + 2 tq + x, elements gq d/8 + 2 t + (0, 1)
+  // ---- the warps' partial results: row 8 nr + 2 tq + x, two neighbouring elements from every M tile
 #pragma unroll
   for (int nr = 0; nr < NR; ++nr) {
 #pragma unroll
@@ -464,7 +516,7 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const CacheA
       }
 #pragma unroll
       for (int t = 0; t < KS; ++t)
-        *reinterpret_cast<float2*>(&po[warp][row][gq * (HD / 8) + 2 * t]) = make_float2(o[t][nr][x], o[t][nr][x + 2]);
+        *reinterpret_cast<float2*>(&po[warp][row][C::v_element(gq, t)]) = make_float2(o[t][nr][x], o[t][nr][x + 2]);
     }
   }
   __syncthreads();
@@ -546,11 +598,14 @@ int decode_launch(CacheAttnArgs a, int64_t max_keys, int num_sms, cudaStream_t s
   const int64_t ctas = int64_t(tiles) * a.c.kv_heads * a.s.n_seqs;
   const int64_t keys = a.window > 0 ? std::min<int64_t>(max_keys, int64_t(a.window) + a.sinks + a.s.max_rows) : max_keys;
   int splits = 1;
-  while (splits < kMaxSplits && ctas * splits < 12 * num_sms && splits * 2 * kWarps * kChunk * 2 <= keys) splits *= 2;
+  while (splits < kMaxSplits && ctas * splits < 6 * num_sms && splits * 2 * kWarps * kChunk * 2 <= keys) splits *= 2;
   a.splits = splits;
   auto kernel = decode_attention_kernel<HD, T, E4M3, NR>;
+  constexpr int SMEM = decode_smem_bytes<HD, E4M3, NR>();
+  const int st = raise_smem_limit(reinterpret_cast<const void*>(kernel), SMEM, "decode_attention_kernel: shared memory");
+  if (st != PLM_OK) return st;
   const dim3 grid(splits, unsigned(tiles * a.c.kv_heads), unsigned(a.s.n_seqs));
-  return check_cuda(launch_cluster(kernel, grid, dim3(kThreads), 0, stream, true, splits, 1, a), "decode_attention_kernel");
+  return check_cuda(launch_cluster(kernel, grid, dim3(kThreads), SMEM, stream, true, splits, 1, a), "decode_attention_kernel");
 }
 
 template <int HD, typename T>
