@@ -337,6 +337,8 @@ typedef struct plm_cache_attention_desc {
   int32_t sinks;            /* first tokens that stay visible behind the window */
   const int32_t* depth;     /* nullable: [rows] relative to the row's context */
   const int32_t* own_start; /* nullable, with depth: [rows] */
+  void* workspace;          /* device memory, 16-byte aligned, for this call alone until it has run */
+  int64_t workspace_bytes;  /* at least what plm_cache_attention_workspace says */
   plm_paged_cache cache;
   plm_sequences seqs;
 } plm_cache_attention_desc;
@@ -484,8 +486,11 @@ int plm_attention(plm_ctx* ctx, const plm_attention_desc* desc, void* stream);
 int plm_kv_append(plm_ctx* ctx, const plm_kv_append_desc* desc, void* stream);
 int plm_add_rmsnorm(plm_ctx* ctx, const plm_add_rmsnorm_desc* desc, void* stream);
 int plm_commit(plm_ctx* ctx, const plm_commit_desc* desc, void* stream);
-/* Both use no memory of the context but its error word, so calls on several streams and captured graphs may overlap. */
+/* Both use no memory of the context but its error word, so calls on several streams and captured graphs may overlap as
+ * long as each has a workspace of its own. plm_cache_attention_workspace gives the bytes a call of this shape needs, 0 for
+ * none (host only; desc's workspace fields are not read). */
 int plm_cache_append(plm_ctx* ctx, const plm_cache_append_desc* desc, void* stream);
+int plm_cache_attention_workspace(plm_ctx* ctx, const plm_cache_attention_desc* desc, int64_t* bytes);
 int plm_cache_attention(plm_ctx* ctx, const plm_cache_attention_desc* desc, void* stream);
 
 /* ---- round engine ---- */

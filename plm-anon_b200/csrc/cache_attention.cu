@@ -623,9 +623,13 @@ int attention_launch(const CacheAttnArgs& a, int kind, int64_t max_keys, int num
 
 using namespace plm;
 
-extern "C" int plm_cache_attention(plm_ctx* ctx, const plm_cache_attention_desc* d, void* stream) {
+namespace {
+
+// Validates a call and fills the argument block.
+int attention_arguments(plm_ctx* ctx, const plm_cache_attention_desc* d, CacheAttnArgs* out, int64_t* max_keys) {
   if (ctx == nullptr || d == nullptr) return fail(PLM_ERR_INVALID, "plm_cache_attention: null argument");
-  CacheAttnArgs a = {};
+  CacheAttnArgs& a = *out;
+  a = {};
   int st = cache_arguments("plm_cache_attention", d->cache, d->seqs, d->dtype, d->rows, &a.c, &a.s);
   if (st != PLM_OK) return st;
   const int hd = d->cache.head_dim;
@@ -656,12 +660,43 @@ extern "C" int plm_cache_attention(plm_ctx* ctx, const plm_cache_attention_desc*
   a.sinks = d->sinks;
   a.depth = d->depth;
   a.own_start = d->own_start;
+  a.workspace = d->workspace;
   a.err = ctx->err;
   a.s.max_rows = std::min(a.s.max_rows, a.s.rows);  // a larger bound only widens the grid
-  const int64_t max_keys = d->seqs.max_keys > 0 ? std::min(d->seqs.max_keys, a.s.max_tokens) : a.s.max_tokens;
+  *max_keys = d->seqs.max_keys > 0 ? std::min(d->seqs.max_keys, a.s.max_tokens) : a.s.max_tokens;
+  return PLM_OK;
+}
+
+size_t workspace_bytes(const plm_ctx* ctx, const plm_cache_attention_desc* d, const CacheAttnArgs& a, int64_t max_keys) {
+  return decode_takes(a) ? decode_workspace(a, d->cache.kind, d->cache.head_dim, max_keys, ctx->num_sms) : 0;
+}
+
+}  // namespace
+
+extern "C" int plm_cache_attention_workspace(plm_ctx* ctx, const plm_cache_attention_desc* d, int64_t* bytes) {
+  CacheAttnArgs a;
+  int64_t max_keys = 0;
+  if (bytes == nullptr) return fail(PLM_ERR_INVALID, "plm_cache_attention_workspace: null argument");
+  const int st = attention_arguments(ctx, d, &a, &max_keys);
+  if (st != PLM_OK) return st;
+  *bytes = int64_t(workspace_bytes(ctx, d, a, max_keys));
+  return PLM_OK;
+}
+
+extern "C" int plm_cache_attention(plm_ctx* ctx, const plm_cache_attention_desc* d, void* stream) {
+  CacheAttnArgs a;
+  int64_t max_keys = 0;
+  const int st = attention_arguments(ctx, d, &a, &max_keys);
+  if (st != PLM_OK) return st;
+  const int64_t needs = int64_t(workspace_bytes(ctx, d, a, max_keys));
+  if (needs > 0 && (d->workspace == nullptr || !aligned16(d->workspace) || d->workspace_bytes < needs))
+    return fail(PLM_ERR_INVALID, "plm_cache_attention: a 16-byte aligned workspace of %lld bytes is needed (%lld given)",
+                (long long)needs, (long long)(d->workspace ? d->workspace_bytes : 0));
   DeviceScope scope(ctx->device);
   if (scope.status() != PLM_OK) return scope.status();
   cudaStream_t on = static_cast<cudaStream_t>(stream);
+  const int hd = d->cache.head_dim;
+  if (decode_takes(a)) return decode_attention(a, d->cache.kind, d->dtype, hd, max_keys, ctx->num_sms, on);
   if (d->dtype == PLM_F16)
     return hd == 128 ? attention_launch<128, __half>(a, d->cache.kind, max_keys, ctx->num_sms, on)
                      : attention_launch<64, __half>(a, d->cache.kind, max_keys, ctx->num_sms, on);

@@ -17,7 +17,15 @@ struct CacheAttnArgs {
   int window, sinks;
   const int32_t *depth, *own_start;
   int splits;        // CTAs of a cluster that share a sequence's keys
+  void* workspace;
   int* err;
 };
+
+// Sequences of at most 16 packed rows (cache_decode.cu): whether all of a call's are, the bytes of workspace the call
+// needs, and the launch.
+bool decode_takes(const CacheAttnArgs& a);
+size_t decode_workspace(const CacheAttnArgs& a, int kind, int head_dim, int64_t max_keys, int num_sms);
+int decode_attention(const CacheAttnArgs& a, int kind, int dtype, int head_dim, int64_t max_keys, int num_sms,
+                     cudaStream_t stream);
 
 }  // namespace plm

@@ -159,6 +159,14 @@ def _output(like: torch.Tensor, stream) -> torch.Tensor:
         return torch.empty(like.shape, dtype=like.dtype, device=like.device)
 
 
+def _scratch(size: int, device: torch.device, stream) -> torch.Tensor:
+    """Bytes for one call, from the allocator of the stream that it runs on (a captured call's from its graph's pool)."""
+    if stream is None:
+        return torch.empty(size, dtype=torch.uint8, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(size, dtype=torch.uint8, device=device)
+
+
 def append(ctx: native.Context, cache: PagedCache, seqs: Sequences, k: torch.Tensor, v: torch.Tensor, *,
            q: torch.Tensor | None = None, q_out: torch.Tensor | None = None, cos_sin: torch.Tensor | None = None,
            positions: torch.Tensor | None = None, stream=None) -> torch.Tensor | None:
@@ -229,6 +237,10 @@ def attention(ctx: native.Context, cache: PagedCache, seqs: Sequences, q: torch.
         dtype=code, rows=rows, q=q.data_ptr(), q_stride=q_stride, out=out.data_ptr(), out_stride=out_stride,
         num_heads=heads, scale=scale or 0.0, window=window, sinks=sinks, depth=depth_ptr, own_start=own_ptr,
         cache=cache.desc, seqs=seqs.desc)
+    size = native.cache_attention_workspace(ctx, desc)
+    if size:
+        workspace = _scratch(size, device, stream)
+        desc.workspace, desc.workspace_bytes = workspace.data_ptr(), size
     on = (stream if stream is not None else torch.cuda.current_stream(device)).cuda_stream
     native.check(native.library().plm_cache_attention(ctx.handle, ctypes.byref(desc), on), "plm_cache_attention")
     return out

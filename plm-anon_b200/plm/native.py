@@ -123,8 +123,8 @@ class CacheAppendDesc(ctypes.Structure):
 class CacheAttentionDesc(ctypes.Structure):
     _fields_ = [("dtype", c_int32), ("rows", c_int32), ("q", c_void_p), ("q_stride", c_int64), ("out", c_void_p),
                 ("out_stride", c_int64), ("num_heads", c_int32), ("scale", ctypes.c_float), ("window", c_int32),
-                ("sinks", c_int32), ("depth", c_void_p), ("own_start", c_void_p), ("cache", PagedCacheDesc),
-                ("seqs", SequencesDesc)]
+                ("sinks", c_int32), ("depth", c_void_p), ("own_start", c_void_p), ("workspace", c_void_p),
+                ("workspace_bytes", c_int64), ("cache", PagedCacheDesc), ("seqs", SequencesDesc)]
 
 
 class ModelDesc(ctypes.Structure):
@@ -191,6 +191,7 @@ _SIGNATURES: dict[str, list] = {
     "plm_add_rmsnorm": [c_void_p, POINTER(AddRmsNormDesc), c_void_p],
     "plm_commit": [c_void_p, POINTER(CommitDesc), c_void_p],
     "plm_cache_append": [c_void_p, POINTER(CacheAppendDesc), c_void_p],
+    "plm_cache_attention_workspace": [c_void_p, POINTER(CacheAttentionDesc), POINTER(c_int64)],
     "plm_cache_attention": [c_void_p, POINTER(CacheAttentionDesc), c_void_p],
     "plm_icdf_decode": [c_void_p, POINTER(IcdfDesc), c_void_p],
     "plm_block_schedule": [c_int32, c_int32, c_int32, c_int32, POINTER(c_int32), c_int32, POINTER(c_int32),
@@ -328,6 +329,14 @@ def commit(ctx: Context, desc: CommitDesc, stream=None) -> None:
 def cache_append(ctx: Context, desc: CacheAppendDesc, stream=None) -> None:
     """Enqueue plm_cache_append (``plm.cache.append`` takes tensors and checks them)."""
     check(library().plm_cache_append(ctx.handle, ctypes.byref(desc), stream_handle(stream)), "plm_cache_append")
+
+
+def cache_attention_workspace(ctx: Context, desc: CacheAttentionDesc) -> int:
+    """Bytes of workspace that a plm_cache_attention call of this shape needs."""
+    size = c_int64(0)
+    check(library().plm_cache_attention_workspace(ctx.handle, ctypes.byref(desc), ctypes.byref(size)),
+          "plm_cache_attention_workspace")
+    return size.value
 
 
 def cache_attention(ctx: Context, desc: CacheAttentionDesc, stream=None) -> None:
