@@ -16,7 +16,7 @@ struct CacheAttnArgs {
   float scale_log2;  // of the scores, in units of log2
   int window, sinks;
   const int32_t *depth, *own_start;
-  int splits;        // CTAs of a cluster that share a sequence's keys
+  int splits;        // CTAs that share a unit's keys (cache_prefill.cu)
   void* workspace;
   int* err;
 };
@@ -27,5 +27,9 @@ bool decode_takes(const CacheAttnArgs& a);
 size_t decode_workspace(const CacheAttnArgs& a, int kind, int head_dim, int64_t max_keys, int num_sms);
 int decode_attention(const CacheAttnArgs& a, int kind, int dtype, int head_dim, int64_t max_keys, int num_sms,
                      cudaStream_t stream);
+// All others (cache_prefill.cu).
+size_t prefill_workspace(const CacheAttnArgs& a, int head_dim, int64_t max_keys, int num_sms);
+int prefill_attention(const CacheAttnArgs& a, int kind, int dtype, int head_dim, int64_t max_keys, int num_sms,
+                      cudaStream_t stream);
 
 }  // namespace plm
