@@ -34,7 +34,7 @@ constexpr int kTile = 128;  // rows of a stream, and keys
 constexpr int kUnit = 2 * kTile;
 constexpr int kRoleThreads = 128;
 constexpr int kPrefillThreads = 5 * kRoleThreads;
-constexpr int kFactorSlots = 4;
+constexpr int kScaleSlots = 4;
 constexpr uint32_t kTmemColumns = 512;
 
 template <int HD>
@@ -43,14 +43,17 @@ struct PrefillSmem {
   static constexpr int Q = 0;
   static constexpr int K = 2 * TILE;
   static constexpr int V = 4 * TILE;
-  static constexpr int FACTORS = 6 * TILE;     // [slot][k scale, log2 v scale, 1 / v scale][128]
-  static constexpr int BARRIERS = FACTORS + kFactorSlots * 3 * kTile * 4;
-  static constexpr int BYTES = BARRIERS + 256 + 1024;  // and the alignment's slack
+  static constexpr int SCALES = 6 * TILE;      // [slot] TileScales
+  static constexpr int FETCH = SCALES + kScaleSlots * 3 * kTile * 4;  // [2] FetchRows
+  static constexpr int BARRIERS = FETCH + 2 * 2176;
+  static constexpr int UNIT = BARRIERS + 256;
+  static constexpr int BYTES = UNIT + 256 + 1024;  // and the alignment's slack
 };
 
 struct PrefillBarriers {
   uint64_t q_ready, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], pv_done[2],
-      factors_full[kFactorSlots];
+      scales_full[kScaleSlots];
+  int one[kScaleSlots];  // whether the tile has one scale
   uint32_t tmem;
   int odd;  // a value that is no number was met in a masked tile
 };
@@ -93,21 +96,35 @@ __device__ __forceinline__ uint64_t umma_desc_transposed(uint32_t smem_addr, uin
   return d;
 }
 // 16 words of every lane into 16 columns of tensor memory.
-__device__ __forceinline__ void tmem_st_16cols(uint32_t taddr, const uint32_t (&r)[16]) {
+__device__ __forceinline__ void tmem_st_16cols(uint32_t taddr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
-__device__ __forceinline__ void tmem_st_32cols(uint32_t taddr, const float (&v)[32]) {
-  uint32_t r[16];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(v[h * 16 + i]);
-    tmem_st_16cols(taddr + h * 16, r);
-  }
+// 32 columns of every lane, to be waited for with tmem_wait_ld.
+__device__ __forceinline__ void tmem_ld_32(uint32_t taddr, float* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+        "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]),
+        "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
+        "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_ld_16cols(uint32_t taddr, float (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+        "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+      : "r"(taddr)
+      : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_proxy_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -125,21 +142,27 @@ __device__ __forceinline__ int tile_at(int row, int vec) {
   return (vec >> 3) * (kTile * 128) + row * 128 + (((vec & 7) ^ (row & 7)) << 4);
 }
 
+// Which key tiles of a CTA each stream works on: with one row tile every second one; with two row tiles the sinks' and
+// those that some of its rows see.
+struct Turns {
+  bool two;
+  int t_begin, t_end;  // the CTA's key tiles
+  int sinks[2], begin[2], end[2];
+  __device__ __forceinline__ bool active(int s, int t) const {
+    if (!two) return ((t - t_begin) & 1) == s;
+    return t < sinks[s] || (t >= begin[s] && t < end[s]);
+  }
+};
+
 // What a CTA works on.
 struct Unit {
   SeqRange r;
-  int seq, head, i0, rows;    // packed rows [i0, i0 + rows)
-  bool two;                   // row tiles
-  TileKeys keys;              // of all its rows, in tiles of 128 keys
-  TileKeys stream_keys[2];    // of a stream's rows
-  int t_begin, t_end;         // this CTA's key tiles
-  // Whether stream s works on key tile t: with two row tiles, unless none of its rows sees a key there.
-  __device__ __forceinline__ bool active(int s, int t) const {
-    if (!two) return ((t - t_begin) & 1) == s;
-    const int kv = keys.key<kTile>(t);
-    return kv < stream_keys[s].end && (kv + kTile > stream_keys[s].lo || kv < stream_keys[s].sinks);
-  }
+  int seq, head, i0, rows;   // packed rows [i0, i0 + rows); rows 0: nothing
+  TileKeys keys;             // of all its rows, in tiles of 128 keys
+  TileKeys stream_keys[2];   // of a stream's rows
+  Turns turns;
 };
+static_assert(sizeof(Unit) <= 256, "unit");
 
 // Unit `index` of the call's rows, or false past the last one. All threads of a warp together.
 __device__ __forceinline__ bool find_unit(const CacheAttnArgs& a, int index, int head, int split, Unit* u) {
@@ -174,7 +197,7 @@ __device__ __forceinline__ bool find_unit(const CacheAttnArgs& a, int index, int
   u->head = head;
   u->i0 = unit * kUnit;
   u->rows = min(kUnit, u->r.n * a.group - u->i0);
-  u->two = u->rows > kTile;
+  const bool two = u->rows > kTile;
   const int j0 = u->i0 / a.group, j1 = (u->i0 + u->rows - 1) / a.group;
   TileKeys t = causal_keys(a, u->r, j0, j1);
   if (a.depth != nullptr) {
@@ -189,29 +212,41 @@ __device__ __forceinline__ bool find_unit(const CacheAttnArgs& a, int index, int
   }
   t.count<kTile>();
   u->keys = u->stream_keys[0] = u->stream_keys[1] = t;
-  if (u->two && a.depth == nullptr) {
-    u->stream_keys[0] = causal_keys(a, u->r, j0, (u->i0 + kTile - 1) / a.group);
-    u->stream_keys[1] = causal_keys(a, u->r, (u->i0 + kTile) / a.group, j1);
+  Turns& turns = u->turns;
+  turns.two = two;
+  turns.t_begin = int(int64_t(split) * t.chunks / a.splits);
+  turns.t_end = int(int64_t(split + 1) * t.chunks / a.splits);
+  for (int s = 0; s < 2; ++s) {
+    turns.sinks[s] = turns.begin[s] = 0;
+    turns.end[s] = t.chunks;
+    if (!two || a.depth != nullptr) continue;
+    const int mid = u->i0 + kTile;
+    const TileKeys k = s == 0 ? causal_keys(a, u->r, j0, (mid - 1) / a.group) : causal_keys(a, u->r, mid / a.group, j1);
+    u->stream_keys[s] = k;
+    const int main = t.sink_chunks - t.lo / kTile;  // from a key's tile to its number
+    turns.sinks[s] = min(t.sink_chunks, (k.sinks + kTile - 1) / kTile);
+    turns.begin[s] = k.sinks > t.lo / kTile * kTile ? t.sink_chunks : main + k.lo / kTile;
+    turns.end[s] = main + (k.end + kTile - 1) / kTile;
   }
-  u->t_begin = int(int64_t(split) * t.chunks / a.splits);
-  u->t_end = int(int64_t(split + 1) * t.chunks / a.splits);
   return true;
 }
 
 // Places of keys in the pages.
+constexpr uint32_t kNoRow = 0xffffffffu;
 struct PageRows {
   const int32_t* table;
-  int page_shift, page_mask, num_pages, kv_heads, head, page_size;
+  int page_shift, page_mask, num_pages, kv_heads, head;
   int* err;
-  // Key kv's row within a plane, in rows of d elements, or -1 where there is none to fetch.
-  __device__ __forceinline__ int64_t row(const TileKeys& t, int kv) const {
-    if (!t.needed(kv)) return -1;
+  // Key kv's row within a plane, in rows of d elements (a plane on the device has fewer than 2^32), or kNoRow where
+  // there is none to fetch.
+  __device__ __forceinline__ uint32_t row(const TileKeys& t, int kv) const {
+    if (!t.needed(kv)) return kNoRow;
     const int page = table[kv >> page_shift];
     if (unsigned(page) >= unsigned(num_pages)) {
       record_error(err, kErrBadIndex);
-      return -1;
+      return kNoRow;
     }
-    return (int64_t(page) * kv_heads + head) * page_size + (kv & page_mask);
+    return (uint32_t(page) * uint32_t(kv_heads) + uint32_t(head)) * uint32_t(page_mask + 1) + uint32_t(kv & page_mask);
   }
 };
 
@@ -235,14 +270,54 @@ __device__ __forceinline__ void drop_non_finite(uint4& x) {
       if (non_finite<T, E4M3>(w[i], at)) w[i] &= ~((E4M3 ? 0xffu : 0xffffu) << ((E4M3 ? 8 : 16) * at));
 }
 
+// What softmax needs to know of a tile of e4m3 keys. Normally the scales of a tile are powers of two within 2^15 of
+// each other, and the codes are brought to the largest one's on the way into shared memory, exactly: then the tile has
+// one scale. Otherwise they stay as they are, and softmax applies the scales key by key.
+struct TileScales {
+  float k[kTile], log_v[kTile], inv_v[kTile];  // by key; where `one`, the first of each is the tile's
+};
+
+// What fetching threads share of a tile (in turns of two).
+struct FetchRows {
+  uint32_t row[2][kTile];
+  float scale[2][kTile];   // e4m3: the largest scale's share that the key's is, or 1 for all
+  float low[4], high[4];   // by warp
+  int odd[4];
+  int abort;               // a wait ran out: the four warps stop together
+};
+static_assert(sizeof(TileScales) == 3 * kTile * 4 && sizeof(FetchRows) <= 2176, "shared memory");
+
+// The scale of a key of e4m3 codes, relative to the tile's largest; whether the tile has one scale. 128 threads, a key
+// each (`live` false: none), `named` their barrier.
+__device__ __forceinline__ bool one_scale(FetchRows* rows, int named, bool live, float scale, float* relative, float* top) {
+  const int tid = threadIdx.x & (kRoleThreads - 1), warp = tid >> 5;
+  const float low = -warp_max(live ? -scale : -INFINITY), high = warp_max(live ? scale : 0.f);
+  const uint32_t bits = __float_as_uint(scale);
+  const bool odd = __any_sync(0xffffffffu, live && ((bits & 0x7fffffu) != 0 || !(scale > 0.f && scale < INFINITY)));
+  if ((tid & 31) == 0) {
+    rows->low[warp] = low;
+    rows->high[warp] = high;
+    rows->odd[warp] = odd ? 1 : 0;
+  }
+  named_barrier_sync(named, kRoleThreads);
+  const float least = fminf(fminf(rows->low[0], rows->low[1]), fminf(rows->low[2], rows->low[3]));
+  *top = fmaxf(fmaxf(rows->high[0], rows->high[1]), fmaxf(rows->high[2], rows->high[3]));
+  const bool one = (rows->odd[0] | rows->odd[1] | rows->odd[2] | rows->odd[3]) == 0 && *top > 0.f && least * 32768.f >= *top;
+  // the quotient of two powers of two
+  *relative = one && live ? __uint_as_float(bits - __float_as_uint(*top) + 0x3f800000u) : 1.f;
+  return one;
+}
+
 // Fetches all key tiles (VALUES false) or value tiles of the CTA into its ring of two: 128 threads.
 template <int HD, typename T, bool E4M3, bool VALUES>
 __device__ __forceinline__ void fetch_tiles(const CacheAttnArgs& a, const Unit& u, uint8_t* smem, PrefillBarriers* bars) {
   using S = PrefillSmem<HD>;
   const int tid = threadIdx.x & (kRoleThreads - 1), lane = tid & 31;
+  constexpr int NAMED = VALUES ? 3 : 2;
   uint64_t* full = VALUES ? bars->v_full : bars->k_full;
   uint64_t* empty = VALUES ? bars->v_empty : bars->k_empty;
   uint8_t* ring = smem + (VALUES ? S::V : S::K);
+  FetchRows* share = reinterpret_cast<FetchRows*>(smem + S::FETCH) + (VALUES ? 1 : 0);
   const uint8_t* plane = static_cast<const uint8_t*>(VALUES ? a.c.v : a.c.k);
   constexpr int ES = E4M3 ? 1 : 2;
   constexpr int VECS = HD * ES / 16;            // 16-byte vectors of a row in the page
@@ -250,160 +325,157 @@ __device__ __forceinline__ void fetch_tiles(const CacheAttnArgs& a, const Unit& 
   constexpr int PASSES = kTile / PER_PASS;
   const int vec = tid % VECS, first = tid / VECS;
   const PageRows rows = {a.s.tables + u.seq * a.s.table_stride, a.c.page_shift, a.c.page_size - 1,
-                                   a.c.num_pages, a.c.kv_heads, u.head, a.c.page_size, a.err};
-  float* factors = reinterpret_cast<float*>(smem + S::FACTORS);
-  auto arrive = [&](uint64_t* bar) {
-    fence_proxy_async_shared();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(bar);
-  };
-  // Values of a masked tile that are no numbers: 16-bit ones are looked for where they have landed.
-  auto landed = [&](int n) {
-    const int t = u.t_begin + n;
-    if constexpr (VALUES && !E4M3) {
-      if (!u.keys.all_seen(u.keys.key<kTile>(t), kTile)) {
+                         a.c.num_pages, a.c.kv_heads, u.head, a.err};
+  const TileKeys keys = u.keys;
+  const int t_begin = u.turns.t_begin, tiles = u.turns.t_end - t_begin;
+  uint32_t next = tiles > 0 ? rows.row(keys, keys.key<kTile>(t_begin) + tid) : kNoRow;
+  for (int n = 0; n < tiles; ++n) {
+    const int kv0 = keys.key<kTile>(t_begin + n);
+    // the rows of this tile's keys for all threads, the next tile's on their way
+    const uint32_t mine = next;
+    share->row[n & 1][tid] = mine;
+    if (n + 1 < tiles) next = rows.row(keys, keys.key<kTile>(t_begin + n + 1) + tid);
+    const bool look = VALUES && !keys.all_seen(kv0, kTile);  // for values that are no numbers
+    uint8_t* dst = ring + (n & 1) * S::TILE;
+    if constexpr (!E4M3) {
+      if (n >= 2 && !warp_wait(empty + (n & 1), ((n >> 1) - 1) & 1, a.err, kErrTimeoutEmpty)) share->abort = 1;
+      named_barrier_sync(NAMED, kRoleThreads);
+      if (share->abort) break;
+#pragma unroll
+      for (int p = 0; p < PASSES; ++p) {
+        const uint32_t from = share->row[n & 1][first + p * PER_PASS];
+        cp_async_16(dst + tile_at(first + p * PER_PASS, vec),
+                    plane + (from == kNoRow ? 0 : size_t(from) * (HD * ES) + vec * 16), from != kNoRow);
+      }
+      cp_async_commit();
+      cp_async_wait<0>();
+      if (look) {
 #pragma unroll 1
         for (int p = 0; p < PASSES; ++p) {
-          uint4* x = reinterpret_cast<uint4*>(ring + (n & 1) * S::TILE + tile_at(first + p * PER_PASS, vec));
+          uint4* x = reinterpret_cast<uint4*>(dst + tile_at(first + p * PER_PASS, vec));
           if (any_non_finite<T, false>(*x)) {
             drop_non_finite<T, false>(*x);
             bars->odd = 1;
           }
         }
       }
-    }
-    arrive(full + (n & 1));
-  };
-  const int tiles = u.t_end - u.t_begin;
-  for (int n = 0; n < tiles; ++n) {
-    const int kv0 = u.keys.key<kTile>(u.t_begin + n);
-    if constexpr (!E4M3) {
-      if (n >= 2 && !warp_wait(empty + (n & 1), ((n >> 1) - 1) & 1, a.err, kErrTimeoutEmpty)) break;
-      uint8_t* dst = ring + (n & 1) * S::TILE;
-#pragma unroll 4
-      for (int p = 0; p < PASSES; ++p) {
-        const int row = first + p * PER_PASS;
-        const int64_t at = rows.row(u.keys, kv0 + row);
-        cp_async_16(dst + tile_at(row, vec), plane + (at < 0 ? 0 : size_t(at) * (HD * ES) + vec * 16), at >= 0);
-      }
-      cp_async_commit();
-      if (n > 0) {
-        cp_async_wait<1>();
-        landed(n - 1);
-      }
     } else {
-      uint4 codes[PASSES];
-#pragma unroll
-      for (int p = 0; p < PASSES; ++p) {
-        const int64_t at = rows.row(u.keys, kv0 + first + p * PER_PASS);
-        codes[p] = make_uint4(0, 0, 0, 0);
-        if (at >= 0) codes[p] = *reinterpret_cast<const uint4*>(plane + size_t(at) * HD + vec * 16);
-      }
-      float ks = 0.f, vs = 1.f;  // the scales of key tid
+      const uint32_t block = mine == kNoRow ? 0 : mine >> a.c.block_shift;  // blocks divide pages: their numbers run on
+      const bool live = mine != kNoRow;
+      const float vs = live ? fmaxf(a.c.v_scale[block], kLeastScale) : 1.f;
+      float relative, v_top;
+      const bool v_one = one_scale(share, NAMED, live, vs, &relative, &v_top);
+      bool in_time = true;
       if constexpr (!VALUES) {
-        const int64_t at = rows.row(u.keys, kv0 + tid);
-        if (at >= 0) {
-          const int64_t block = (at >> a.c.page_shift) * (a.c.page_size >> a.c.block_shift) +
-                                ((at & (a.c.page_size - 1)) >> a.c.block_shift);
-          ks = a.c.k_scale[block];
-          vs = fmaxf(a.c.v_scale[block], kLeastScale);
+        const float ks = live ? a.c.k_scale[block] : 1.f;
+        float k_top;
+        named_barrier_sync(NAMED, kRoleThreads);
+        const bool k_one = one_scale(share, NAMED, live, ks, &relative, &k_top);
+        in_time = n < 2 || warp_wait(empty + (n & 1), ((n >> 1) - 1) & 1, a.err, kErrTimeoutEmpty);
+        if (in_time) {
+          // The scales' slot: its last readers, the softmax of tile n - 4, are done. The products Q K of tiles n - 3 and
+          // n - 2 have run, and a stream's products start only when its softmax of the tile before is over.
+          const int slot = n % kScaleSlots;
+          TileScales& scales = reinterpret_cast<TileScales*>(smem + S::SCALES)[slot];
+          const float v = v_one ? v_top : vs;
+          scales.k[tid] = k_one ? k_top : ks;
+          scales.log_v[tid] = lg2(v);
+          scales.inv_v[tid] = rcp(v);
+          if (tid == 0) bars->one[slot] = k_one && v_one ? 1 : 0;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bars->scales_full + slot);
         }
+      } else {
+        in_time = n < 2 || warp_wait(empty + (n & 1), ((n >> 1) - 1) & 1, a.err, kErrTimeoutEmpty);
       }
-      if (n >= 2 && !warp_wait(empty + (n & 1), ((n >> 1) - 1) & 1, a.err, kErrTimeoutEmpty)) break;
-      if constexpr (!VALUES) {
-        // Their slot's last readers, the softmax of tile n - 4, are done: the products Q K of tiles n - 3 and n - 2 have
-        // run, and a stream's products start only when its softmax of the tile before is over.
-        float* f = factors + (n % kFactorSlots) * 3 * kTile;
-        f[tid] = ks;
-        f[kTile + tid] = lg2(vs);
-        f[2 * kTile + tid] = rcp(vs);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bars->factors_full + n % kFactorSlots);
-      }
-      uint8_t* dst = ring + (n & 1) * S::TILE;
-      const bool look = VALUES && !u.keys.all_seen(kv0, kTile);
+      if (!in_time) share->abort = 1;
+      share->scale[n & 1][tid] = relative;
+      named_barrier_sync(NAMED, kRoleThreads);
+      if (share->abort) break;
+      constexpr int HELD = 4;  // vectors of codes a thread has on their way at once
+#pragma unroll 1
+      for (int p0 = 0; p0 < PASSES; p0 += HELD) {
+        uint4 codes[HELD];
 #pragma unroll
-      for (int p = 0; p < PASSES; ++p) {
-        if (look && any_non_finite<T, true>(codes[p])) {
-          drop_non_finite<T, true>(codes[p]);
-          bars->odd = 1;
+        for (int p = 0; p < HELD; ++p) {
+          const uint32_t from = share->row[n & 1][first + (p0 + p) * PER_PASS];
+          codes[p] = make_uint4(0, 0, 0, 0);
+          if (from != kNoRow) codes[p] = *reinterpret_cast<const uint4*>(plane + size_t(from) * HD + vec * 16);
         }
-        const uint32_t w[4] = {codes[p].x, codes[p].y, codes[p].z, codes[p].w};
-        uint32_t h[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          h[2 * i] = e4m3x2_to_f16x2(uint16_t(w[i]));
-          h[2 * i + 1] = e4m3x2_to_f16x2(uint16_t(w[i] >> 16));
+        for (int p = 0; p < HELD; ++p) {
+          if (look && any_non_finite<T, true>(codes[p])) {
+            drop_non_finite<T, true>(codes[p]);
+            bars->odd = 1;
+          }
+          const int row = first + (p0 + p) * PER_PASS;
+          const __half2 by = __float2half2_rn(share->scale[n & 1][row]);
+          const uint32_t w[4] = {codes[p].x, codes[p].y, codes[p].z, codes[p].w};
+          uint32_t h[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t x = e4m3x2_to_f16x2(uint16_t(w[i / 2] >> (16 * (i & 1))));
+            const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&x), by);
+            h[i] = *reinterpret_cast<const uint32_t*>(&y);
+          }
+          *reinterpret_cast<uint4*>(dst + tile_at(row, 2 * vec)) = make_uint4(h[0], h[1], h[2], h[3]);
+          *reinterpret_cast<uint4*>(dst + tile_at(row, 2 * vec + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
         }
-        const int row = first + p * PER_PASS;
-        *reinterpret_cast<uint4*>(dst + tile_at(row, 2 * vec)) = make_uint4(h[0], h[1], h[2], h[3]);
-        *reinterpret_cast<uint4*>(dst + tile_at(row, 2 * vec + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
       }
-      arrive(full + (n & 1));
     }
-  }
-  if constexpr (!E4M3) {
-    cp_async_wait<0>();
-    if (tiles > 0) landed(tiles - 1);
+    fence_proxy_async_shared();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(full + (n & 1));
   }
 }
 
-// Issues all products: one warp, its first lane.
+// Issues all products: one thread, so that nothing of its warp has to be brought together again after a wait.
 template <int HD, bool BF16>
-__device__ __forceinline__ void issue_products(const CacheAttnArgs& a, const Unit& u, uint8_t* smem, PrefillBarriers* bars) {
+__device__ __forceinline__ void issue_products(const CacheAttnArgs& a, const Turns& turns, uint8_t* smem,
+                                               PrefillBarriers* bars) {
   using S = PrefillSmem<HD>;
   constexpr uint32_t QK = umma_idesc_f16(kTile, kTile, BF16);
   constexpr uint32_t PV = umma_idesc_f16(kTile, HD, BF16) | (1u << 16);  // B transposed
   constexpr int PANEL = kTile * 128;
-  const int lane = threadIdx.x & 31;
+  constexpr int STEP = S::TILE >> 4;  // a tile, in a descriptor's units
   const uint32_t tmem = bars->tmem;
-  const uint32_t q_addr = smem_u32(smem + S::Q), k_addr = smem_u32(smem + S::K), v_addr = smem_u32(smem + S::V);
-  const int tiles = u.t_end - u.t_begin;
+  const uint64_t q_desc = umma_desc_sw128(smem_u32(smem + S::Q)), k_desc = umma_desc_sw128(smem_u32(smem + S::K));
+  const uint64_t v_desc = umma_desc_transposed(smem_u32(smem + S::V), PANEL);
+  const bool two = turns.two;
+  const int t_begin = turns.t_begin, tiles = turns.t_end - t_begin;
   bool ok = true;
-  auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
-    if (!ok) return;
-    int got = 1;
-    if (lane == 0) got = mbar_wait(bar, parity, a.err, code) ? 1 : 0;
-    ok = __shfl_sync(0xffffffffu, got, 0) != 0;
-  };
-  auto users = [&](int n) { return (u.active(0, u.t_begin + n) ? 1 : 0) + (u.active(1, u.t_begin + n) ? 1 : 0); };
-  auto after = [&](int s, int n) {  // the stream's next tile from n on
-    while (n < tiles && !u.active(s, u.t_begin + n)) ++n;
-    return n;
-  };
+  auto wait = [&](uint64_t* bar, uint32_t parity, int code) { ok = ok && mbar_wait(bar, parity, a.err, code); };
   auto scores = [&](int s, int n) {
     wait(bars->k_full + (n & 1), (n >> 1) & 1, kErrTimeoutFull);
     if (!ok) return;
     tc_fence_after();
-    if (lane == 0) {
-      const uint32_t q = q_addr + (u.two ? s : 0) * S::TILE, k = k_addr + (n & 1) * S::TILE;
+    const uint64_t q = q_desc + (two ? s * STEP : 0), k = k_desc + (n & 1) * STEP;
 #pragma unroll
-      for (int x = 0; x < HD / 16; ++x) {
-        const uint32_t at = (x >> 2) * PANEL + (x & 3) * 32;
-        umma_f16(tmem + s * kTile, umma_desc_sw128(q + at), umma_desc_sw128(k + at), QK, x > 0 ? 1u : 0u);
-      }
-      umma_commit(bars->s_full + s);
-      umma_commit(bars->k_empty + (n & 1));
-      if (users(n) == 1) umma_commit(bars->k_empty + (n & 1));  // the other stream has no use for it
+    for (int x = 0; x < HD / 16; ++x) {
+      const int at = ((x >> 2) * PANEL + (x & 3) * 32) >> 4;
+      umma_f16(tmem + s * kTile, q + at, k + at, QK, x > 0 ? 1u : 0u);
     }
-    __syncwarp();
+    umma_commit(bars->s_full + s);
+    umma_commit(bars->k_empty + (n & 1));
+    if (!turns.active(1 - s, t_begin + n)) umma_commit(bars->k_empty + (n & 1));  // the other stream has no use for it
   };
   auto values = [&](int s, int n, int count) {
     wait(bars->v_full + (n & 1), (n >> 1) & 1, kErrTimeoutFull);
     wait(bars->p_ready + s, count & 1, kErrTimeoutPeer);
     if (!ok) return;
     tc_fence_after();
-    if (lane == 0) {
-      const uint32_t v = v_addr + (n & 1) * S::TILE;
+    const uint64_t v = v_desc + (n & 1) * STEP;
 #pragma unroll
-      for (int x = 0; x < kTile / 16; ++x)
-        umma_f16_ts(tmem + 2 * kTile + s * kTile, tmem + s * kTile + x * 8, umma_desc_transposed(v + x * 2048, PANEL), PV,
-                    count > 0 || x > 0 ? 1u : 0u);
-      umma_commit(bars->pv_done + s);
-      umma_commit(bars->v_empty + (n & 1));
-      if (users(n) == 1) umma_commit(bars->v_empty + (n & 1));
-    }
-    __syncwarp();
+    for (int x = 0; x < kTile / 16; ++x)
+      umma_f16_ts(tmem + 2 * kTile + s * kTile, tmem + s * kTile + x * 8, v + ((x * 2048) >> 4), PV,
+                  count > 0 || x > 0 ? 1u : 0u);
+    umma_commit(bars->pv_done + s);
+    umma_commit(bars->v_empty + (n & 1));
+    if (!turns.active(1 - s, t_begin + n)) umma_commit(bars->v_empty + (n & 1));
+  };
+  auto after = [&](int s, int n) {  // the stream's next tile from n on
+    while (n < tiles && !turns.active(s, t_begin + n)) ++n;
+    return n;
   };
   wait(&bars->q_ready, 0, kErrTimeoutPeer);
   int at[2] = {after(0, 0), after(1, 0)}, count = 0;
@@ -434,10 +506,12 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
   grid_dependency_wait();
   allow_dependents();
   const int split = blockIdx.x % a.splits, index = blockIdx.x / a.splits;
-  Unit u;
-  if (!find_unit(a, index / a.c.kv_heads, index % a.c.kv_heads, split, &u)) {
-    if (a.splits > 1 && split == 0 && tid == 0) static_cast<SplitUnit*>(a.workspace)[index].rows = 0;
-    return;
+  const Unit& u = *reinterpret_cast<const Unit*>(smem + S::UNIT);
+  if (warp == 1) {
+    Unit found;
+    found.rows = 0;
+    find_unit(a, index / a.c.kv_heads, index % a.c.kv_heads, split, &found);
+    if (lane == 0) *reinterpret_cast<Unit*>(smem + S::UNIT) = found;
   }
   if (tid == 0) {
     mbar_init(&bars->q_ready, 8);
@@ -450,9 +524,15 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
       mbar_init(bars->p_ready + i, 4);
       mbar_init(bars->pv_done + i, 1);
     }
-    for (int i = 0; i < kFactorSlots; ++i) mbar_init(bars->factors_full + i, 4);
+    for (int i = 0; i < kScaleSlots; ++i) mbar_init(bars->scales_full + i, 4);
     bars->odd = 0;
+    for (int i = 0; i < 2; ++i) reinterpret_cast<FetchRows*>(smem + S::FETCH)[i].abort = 0;
     fence_barrier_init();
+  }
+  __syncthreads();
+  if (u.rows == 0) {  // past the last unit
+    if (a.splits > 1 && split == 0 && tid == 0) static_cast<SplitUnit*>(a.workspace)[index].rows = 0;
+    return;
   }
   if (warp == 0) tmem_alloc(&bars->tmem, kTmemColumns);
   tc_fence_before();
@@ -460,26 +540,29 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
   tc_fence_after();
   const uint32_t tmem = bars->tmem;
 
-  // Registers: 96 a thread at launch, 5 x 96 = 480 for the five groups of four warps: 2 x 160 + 2 x 56 + 48 = 480.
+  // Registers: 96 a thread at launch, 5 x 96 = 480 for the five groups of four warps: 2 x 168 + 2 x 48 + 48 = 480.
   const int role = tid / kRoleThreads;
   if (role == 2) {
-    registers_dec<56>();
+    registers_dec<48>();
     fetch_tiles<HD, T, E4M3, false>(a, u, smem, bars);
   } else if (role == 3) {
-    registers_dec<56>();
+    registers_dec<48>();
     fetch_tiles<HD, T, E4M3, true>(a, u, smem, bars);
   } else if (role == 4) {
     registers_dec<48>();
-    if (warp == 16) issue_products<HD, std::is_same<M, __nv_bfloat16>::value>(a, u, smem, bars);
+    if (tid == 4 * kRoleThreads) {
+      const Turns turns = u.turns;
+      issue_products<HD, std::is_same<M, __nv_bfloat16>::value>(a, turns, smem, bars);
+    }
   } else {
-    registers_inc<160>();
+    registers_inc<168>();
     const int stream = role;
     float m = -INFINITY, l = 0.f;
     int done = 0;  // key tiles this stream has worked on
     bool ok = true;
     const uint32_t t_lane = tmem + (uint32_t((warp & 3) * 32) << 16);
     const int row = tid & (kRoleThreads - 1);                       // of the stream's tile
-    const int i = u.i0 + (u.two && stream == 1 ? kTile : 0) + row;  // packed row
+    const int i = u.i0 + (u.turns.two && stream == 1 ? kTile : 0) + row;  // packed row
     const bool live = i < u.i0 + u.rows;
     // ---- the row's query into shared memory (with one row tile, stream 0's threads bring it)
     float q_scale = a.scale_log2;
@@ -499,7 +582,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
       up = power_of_two_f32(-e);
       q_scale *= power_of_two_f32(e);
     }
-    if (u.two || stream == 0) {
+    if (u.turns.two || stream == 0) {
       uint8_t* dst = smem + S::Q + stream * S::TILE;
 #pragma unroll 4
       for (int vec = 0; vec < HD / 8; ++vec) {
@@ -517,98 +600,150 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
     __syncwarp();
     if (lane == 0) mbar_arrive(&bars->q_ready);
     const RowMask mask = live ? row_mask(a, u.r, i / a.group) : no_row();
-    const TileKeys& keys = u.stream_keys[stream];
-    const float* factors = reinterpret_cast<const float*>(smem + S::FACTORS);
+    const Turns turns = u.turns;
+    const int full_lo = u.stream_keys[stream].full_lo, full_end = u.stream_keys[stream].full_end,
+              full_sinks = u.stream_keys[stream].sinks;
     const uint32_t t_s = t_lane + stream * kTile, t_o = t_lane + 2 * kTile + stream * kTile;
 
-    for (int n = 0; n < u.t_end - u.t_begin; ++n) {
-      if (!u.active(stream, u.t_begin + n)) continue;
-      const int kv0 = u.keys.key<kTile>(u.t_begin + n);
-      const bool full = keys.all_seen(kv0, kTile);
-      const float* f = factors + (n % kFactorSlots) * 3 * kTile;
-      ok = (!E4M3 || warp_wait(bars->factors_full + n % kFactorSlots, (n / kFactorSlots) & 1, a.err, kErrTimeoutFull)) &&
+    for (int n = 0; n < turns.t_end - turns.t_begin; ++n) {
+      if (!turns.active(stream, turns.t_begin + n)) continue;
+      const int kv0 = u.keys.key<kTile>(turns.t_begin + n);
+      const bool full = kv0 + kTile <= full_end && (kv0 >= full_lo || kv0 + kTile <= full_sinks);
+      const int slot = n % kScaleSlots;
+      ok = (!E4M3 || warp_wait(bars->scales_full + slot, (n / kScaleSlots) & 1, a.err, kErrTimeoutFull)) &&
            warp_wait(bars->s_full + stream, done & 1, a.err, kErrTimeoutDone);
       if (!ok) break;
       tc_fence_after();
-      // Scores of 32 keys in units of log2.
-      auto load_scores = [&](int c, float(&x)[32]) {
-        tmem_ld_32cols(t_s + c, x);
-        if constexpr (E4M3) {
+      // A score x counts as x by + add, in units of log2 and with its value's scale in it; a weight w as w inv_v in l.
+      const TileScales& scales = reinterpret_cast<const TileScales*>(smem + S::SCALES)[slot];
+      float by = q_scale, add = 0.f, inv_v = 1.f;  // by is above 0, so that -inf by stays -inf
+      const bool one = !E4M3 || bars->one[slot] != 0;
+      if (E4M3 && one) {
+        by *= scales.k[0];
+        add = scales.log_v[0];
+        inv_v = scales.inv_v[0];
+      }
+      by = fmaxf(by, 1.17549435e-38f);
+      auto hide = [&](int c, float* x, int count) {  // scores of keys c.. of the tile that the row does not see
+        const int last = mask.last - kv0 - c, first = mask.first - kv0 - c, sinks = a.sinks - kv0 - c;
+        if (a.depth == nullptr) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            const float4 ks = *reinterpret_cast<const float4*>(f + c + e);
-            const float4 lv = *reinterpret_cast<const float4*>(f + kTile + c + e);
-            x[e] = fmaf(x[e] * q_scale, ks.x, lv.x);
-            x[e + 1] = fmaf(x[e + 1] * q_scale, ks.y, lv.y);
-            x[e + 2] = fmaf(x[e + 2] * q_scale, ks.z, lv.z);
-            x[e + 3] = fmaf(x[e + 3] * q_scale, ks.w, lv.w);
-          }
+          for (int e = 0; e < count; ++e)
+            if (!((e <= last) & ((e >= first) | (e < sinks)))) x[e] = -INFINITY;
         } else {
+          const int own_first = mask.own_first - kv0 - c, own_last = mask.own_last - kv0 - c;
 #pragma unroll
-          for (int e = 0; e < 32; ++e) x[e] *= q_scale;
-        }
-        if (!full) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (!mask.sees(kv0 + c + e, a.sinks)) x[e] = -INFINITY;
+          for (int e = 0; e < count; ++e)
+            if (!(((e <= last) & ((e >= first) | (e < sinks))) | ((e >= own_first) & (e <= own_last)))) x[e] = -INFINITY;
         }
       };
-      float top = -INFINITY;
+      auto largest = [&](const float* x, int count) {
+        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < kTile; c += 32) {
-        float x[32];
-        load_scores(c, x);
+        for (int e = 0; e < count; e += 8)
 #pragma unroll
-        for (int e = 0; e < 32; ++e) top = fmaxf(top, x[e]);
-      }
-      if (__any_sync(0xffffffffu, top > m + kLazy)) {
+          for (int y = 0; y < 4; ++y) tops[y] = fmaxf(fmaxf(tops[y], x[e + 2 * y]), x[e + 2 * y + 1]);
+        return fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+      };
+      // A row's maximum to `top` (in units of log2), O and l with it.
+      auto raise = [&](float top) {
         top = fmaxf(top, m);
         const float keep = ex2(m - (top == -INFINITY ? 0.f : top));
         m = top;
         l *= keep;
-        if (done > 0) {
-          ok = warp_wait(bars->pv_done + stream, (done - 1) & 1, a.err, kErrTimeoutDone);
-          if (!ok) break;
-          tc_fence_after();
+        if (done == 0) return;
+        ok = warp_wait(bars->pv_done + stream, (done - 1) & 1, a.err, kErrTimeoutDone);
+        if (!ok) return;
+        tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < HD; c += 32) {
-            float x[32];
-            tmem_ld_32cols(t_o + c, x);
+        for (int c = 0; c < HD; c += 16) {
+          float y[16];
+          tmem_ld_16cols(t_o + c, y);
+          uint32_t z[16];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) x[e] *= keep;
-            tmem_st_32cols(t_o + c, x);
+          for (int e = 0; e < 16; ++e) z[e] = __float_as_uint(y[e] * keep);
+          tmem_st_16cols(t_o + c, z);
+        }
+      };
+      // The tile's maxima alone: the first tile's, and those of a tile with many scales.
+      auto tile_maximum = [&]() {
+        float top = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < kTile; c += 16) {
+          float x[16];
+          tmem_ld_16cols(t_s + c, x);
+          if (!full) hide(c, x, 16);
+          if (one) {
+            top = fmaxf(top, largest(x, 16));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) top = fmaxf(top, fmaf(x[e] * by, scales.k[c + e], scales.log_v[c + e]));
           }
         }
-      }
-      const float from = m == -INFINITY ? 0.f : m;
+        return !one || top == -INFINITY ? top : fmaf(top, by, add);
+      };
+      if (one) {
+        if (done == 0) raise(tile_maximum());
+        // One pass with the maximum as it is; should it prove too small, it is raised and the pass repeated.
+        uint32_t p[kTile / 2];
+        while (true) {
+          const float from = add - (m == -INFINITY ? 0.f : m);
+          const f32x2 scale2 = pair(by, by), from2 = pair(from, from);
+          f32x2 sums[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+          float top = -INFINITY;
+          float x[2][32];
+          tmem_ld_32(t_s, x[0]);
 #pragma unroll
-      for (int c = 0; c < kTile; c += 32) {
-        float x[32];
-        load_scores(c, x);
-        uint32_t p[16];
-        if constexpr (E4M3) {
+          for (int c = 0; c < kTile; c += 32) {
+            float(&y)[32] = x[(c / 32) & 1];
+            tmem_wait_ld();
+            if (c + 32 < kTile) tmem_ld_32(t_s + c + 32, x[(c / 32 + 1) & 1]);
+            if (!full) hide(c, y, 32);
+            top = fmaxf(top, largest(y, 32));
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            const float4 iv = *reinterpret_cast<const float4*>(f + 2 * kTile + c + e);
-            x[e] = ex2(x[e] - from);
-            x[e + 1] = ex2(x[e + 1] - from);
-            x[e + 2] = ex2(x[e + 2] - from);
-            x[e + 3] = ex2(x[e + 3] - from);
-            l = fmaf(x[e], iv.x, l);
-            l = fmaf(x[e + 1], iv.y, l);
-            l = fmaf(x[e + 2], iv.z, l);
-            l = fmaf(x[e + 3], iv.w, l);
+            for (int e = 0; e < 32; e += 2) {
+              float lo, hi;
+              unpair(fma2(pair(y[e], y[e + 1]), scale2, from2), lo, hi);
+              lo = ex2(lo);
+              hi = ex2(hi);
+              sums[(e >> 1) & 1] = add2(pair(lo, hi), sums[(e >> 1) & 1]);
+              p[(c + e) / 2] = pack2<M>(lo, hi);
+            }
           }
-        } else {
+          top = top == -INFINITY ? top : fmaf(top, by, add);
+          if (!__any_sync(0xffffffffu, top > m + kLazy)) {
+            float lo, hi;
+            unpair(add2(sums[0], sums[1]), lo, hi);
+            l = fmaf(lo + hi, inv_v, l);
+            break;
+          }
+          raise(top);
+          if (!ok) break;
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_st_16cols(t_s + c * 16, p + c * 16);  // over scores that have been read
+      } else {
+        const float top = tile_maximum();
+        if (__any_sync(0xffffffffu, top > m + kLazy)) raise(top);
+        if (!ok) break;
+        const float from = m == -INFINITY ? 0.f : m;
+#pragma unroll 1
+        for (int c = 0; c < kTile; c += 32) {
+          float x[32];
+          tmem_ld_32(t_s + c, x);
+          tmem_wait_ld();
+          if (!full) hide(c, x, 32);
+          uint32_t p[16];
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
-            x[e] = ex2(x[e] - from);
-            l += x[e];
+            x[e] = ex2(fmaf(x[e] * by, scales.k[c + e], scales.log_v[c + e]) - from);
+            l = fmaf(x[e], scales.inv_v[c + e], l);
           }
-        }
 #pragma unroll
-        for (int e = 0; e < 16; ++e) p[e] = pack2<M>(x[2 * e], x[2 * e + 1]);
-        tmem_st_16cols(t_s + c / 2, p);  // over scores that have been read
+          for (int e = 0; e < 16; ++e) p[e] = pack2<M>(x[2 * e], x[2 * e + 1]);
+          tmem_st_16cols(t_s + c / 2, p);
+        }
       }
       tmem_wait_st();
       tc_fence_before();
@@ -624,7 +759,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
     constexpr int LD = HD + 4;  // floats between rows: rows meet different banks
     float* part1 = reinterpret_cast<float*>(smem);  // [128][LD], then (m, l), over queries and keys
     float* ml1 = part1 + kTile * LD;
-    if (!u.two && stream == 1) {
+    if (!u.turns.two && stream == 1) {
 #pragma unroll 1
       for (int c = 0; c < HD; c += 32) {
         float x[32];
@@ -637,9 +772,9 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
       ml1[2 * row + 1] = l;
     }
     named_barrier_sync(1, 2 * kRoleThreads);
-    if (u.two || stream == 0) {
+    if (u.turns.two || stream == 0) {
       float keep0 = 1.f, keep1 = 0.f;
-      if (!u.two) {
+      if (!u.turns.two) {
         const float m1 = ml1[2 * row], top = fmaxf(m, m1), from = top == -INFINITY ? 0.f : top;
         keep0 = ex2(m - from);
         keep1 = ex2(m1 - from);
@@ -671,15 +806,15 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
         if (live && bars->odd) {
           // non-finite values of the masked tiles, added to the rows that see them
           const PageRows rows = {a.s.tables + u.seq * a.s.table_stride, a.c.page_shift, a.c.page_size - 1,
-                                 a.c.num_pages, a.c.kv_heads, u.head, a.c.page_size, nullptr};
+                                 a.c.num_pages, a.c.kv_heads, u.head, nullptr};
 #pragma unroll 1
-          for (int t = u.t_begin; t < u.t_end; ++t) {
+          for (int t = turns.t_begin; t < turns.t_end; ++t) {
             const int kv0 = u.keys.key<kTile>(t);
             if (u.keys.all_seen(kv0, kTile)) continue;
 #pragma unroll 1
             for (int kv = kv0; kv < kv0 + kTile; ++kv) {
-              const int64_t at = mask.sees(kv, a.sinks) ? rows.row(u.keys, kv) : -1;
-              if (at < 0) continue;
+              const uint32_t at = mask.sees(kv, a.sinks) ? rows.row(u.keys, kv) : kNoRow;
+              if (at == kNoRow) continue;
               const uint32_t* w = reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.c.v) +
                                                                     (size_t(at) * HD + c) * (E4M3 ? 1 : 2));
               constexpr int PER = E4M3 ? 4 : 2;
