@@ -10,7 +10,7 @@
 namespace plm {
 
 constexpr int kUnreachable = 1 << 30;  // no key's index: block tables hold less than 2^30 tokens
-constexpr float kLazy = 8.f;           // log2 of how far a weight may pass 1 before its row's maximum is raised
+constexpr float kLazy = 15.f;          // log2 of how far a weight may pass 1 before its row's maximum is raised: f16 holds it
 constexpr float kLeastScale = 7.888609052210118e-31f;  // 2^-100: smaller value scales count as this
 
 // 2^x by the special-function unit (relative error 2^-22; -inf gives +0, NaN stays).

@@ -18,11 +18,11 @@
 // warps meet only at a tile's end.
 //
 // The softmax is online in base 2 with a lazy maximum: a row's m is raised (and O, l rescaled) only when a score passes
-// it by more than 2^8, so most chunks take one vote and no cross-lane maximum; weights stay below 2^8.
+// it by more than 2^15, so most chunks take one vote and no cross-lane maximum; weights stay below 2^15.
 //
 // e4m3 pages: codes become f16 exactly, and their scales never touch a 16-bit number. A key's scale multiplies its
 // scores. A value's scale s enters through w = 2^(score + log2 s - m): O += w code and l += w / s, out = O / l, so that
-// m follows the largest term of the sum, w <= 2^8 whatever the scales are, and rounding w to f16 (2^-11) is relative to
+// m follows the largest term of the sum, w <= 2^15 whatever the scales are, and rounding w to f16 (2^-11) is relative to
 // that term. Queries in bf16 become f16 exactly but for elements below 2^-30 of their row's largest (query_exponent).
 // 16-bit pages: products in the model dtype, w rounded to it, as in round_attention_kernel.
 //

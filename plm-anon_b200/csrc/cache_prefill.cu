@@ -8,15 +8,15 @@
 //     S[128, 128] = Q K^T     tcgen05.mma, both operands in shared memory, S in tensor memory;
 //     P = 2^(S scale - m)     a thread per row: S from tensor memory, P (16 bit) back over S's own columns;
 //     O[128, d] += P V        tcgen05.mma, P from tensor memory, V [key][d] as a transposed operand.
-// The issuing order P0 V, Q0 K', P1 V, Q1 K' lets one stream's two products (4 x 128 x 128 x d flops) run under the other
-// one's softmax. Products of one thread execute in order, so S may be overwritten as soon as the product that reads P
-// has been issued.
+// One thread issues P V and the next Q K' of whichever stream is ready, so one stream's two products (4 x 128 x 128 x d
+// flops) run under the other one's softmax. Products of one thread execute in order, so S may be overwritten as soon as the product
+// that reads P has been issued.
 //
-// Roles: warps 0-3 and 4-7 softmax of stream 0 and 1, warps 8-11 fetch keys, warps 12-15 values (16-bit pages by
-// 16-byte asynchronous copies, e4m3 codes through registers, exactly to f16), warp 16 issues the products. Operands lie
+// Roles: warps 0-3 and 4-7 do the softmax of stream 0 and 1, warps 8-11 fetch keys and values (16-bit pages by 16-byte
+// asynchronous copies, e4m3 codes through registers, exactly to f16), a thread of warp 12 issues the products. Operands lie
 // in 128-byte rows with the 128-byte swizzle, d = 128 in two panels. Every wait is bounded.
 //
-// Softmax: base 2, lazy maximum (O is rescaled only when a score passes m by more than 2^8), scales of e4m3 pages kept
+// Softmax: base 2, lazy maximum (O is rescaled only when a score passes m by more than 2^15), scales of e4m3 pages kept
 // out of 16-bit numbers and queries in bf16 brought to f16 exactly, as cache_decode.cu describes.
 //
 // With too few units for the GPU, several CTAs split a unit's keys; their parts go to the workspace and join_parts_kernel
@@ -33,9 +33,12 @@ namespace {
 constexpr int kTile = 128;  // rows of a stream, and keys
 constexpr int kUnit = 2 * kTile;
 constexpr int kRoleThreads = 128;
-constexpr int kPrefillThreads = 5 * kRoleThreads;
+constexpr int kPrefillThreads = 3 * kRoleThreads + 32;
 constexpr int kScaleSlots = 4;
 constexpr uint32_t kTmemColumns = 512;
+constexpr float kGuess = 4.f;  // log2 of how far the first weights may stay below 1
+
+constexpr int kFetchBytes = 3328;
 
 template <int HD>
 struct PrefillSmem {
@@ -44,8 +47,8 @@ struct PrefillSmem {
   static constexpr int K = 2 * TILE;
   static constexpr int V = 4 * TILE;
   static constexpr int SCALES = 6 * TILE;      // [slot] TileScales
-  static constexpr int FETCH = SCALES + kScaleSlots * 3 * kTile * 4;  // [2] FetchRows
-  static constexpr int BARRIERS = FETCH + 2 * 2176;
+  static constexpr int FETCH = SCALES + kScaleSlots * 3 * kTile * 4;  // FetchRows
+  static constexpr int BARRIERS = FETCH + kFetchBytes;
   static constexpr int UNIT = BARRIERS + 256;
   static constexpr int BYTES = UNIT + 256 + 1024;  // and the alignment's slack
 };
@@ -117,26 +120,16 @@ __device__ __forceinline__ void tmem_ld_32(uint32_t taddr, float* v) {
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_ld_16cols(uint32_t taddr, float (&v)[16]) {
+__device__ __forceinline__ void tmem_ld_16(uint32_t taddr, float (&v)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
       : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
         "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
       : "r"(taddr)
       : "memory");
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_proxy_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void registers_inc() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void registers_dec() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
-
 // Byte offset of 16-byte vector `vec` of row `row` in a tile of 128 rows of d 16-bit elements.
 __device__ __forceinline__ int tile_at(int row, int vec) {
   return (vec >> 3) * (kTile * 128) + row * 128 + (((vec & 7) ^ (row & 7)) << 4);
@@ -145,12 +138,20 @@ __device__ __forceinline__ int tile_at(int row, int vec) {
 // Which key tiles of a CTA each stream works on: with one row tile every second one; with two row tiles the sinks' and
 // those that some of its rows see.
 struct Turns {
-  bool two;
+  int two;             // row tiles: 1 for two
   int t_begin, t_end;  // the CTA's key tiles
-  int sinks[2], begin[2], end[2];
+  int sinks0, begin0, end0, sinks1, begin1, end1;
+  // (Fields by stream, not arrays: an index known only at run time would put them into local memory.)
   __device__ __forceinline__ bool active(int s, int t) const {
     if (!two) return ((t - t_begin) & 1) == s;
-    return t < sinks[s] || (t >= begin[s] && t < end[s]);
+    return t < (s ? sinks1 : sinks0) || (t >= (s ? begin1 : begin0) && t < (s ? end1 : end0));
+  }
+  // The stream's first tile from t on (t_end or more: none).
+  __device__ __forceinline__ int next(int s, int t) const {
+    if (!two) return t + (((t - t_begin) ^ s) & 1);
+    if (t < (s ? sinks1 : sinks0)) return t;
+    t = max(t, s ? begin1 : begin0);
+    return t < (s ? end1 : end0) ? t : t_end;
   }
 };
 
@@ -213,20 +214,23 @@ __device__ __forceinline__ bool find_unit(const CacheAttnArgs& a, int index, int
   t.count<kTile>();
   u->keys = u->stream_keys[0] = u->stream_keys[1] = t;
   Turns& turns = u->turns;
-  turns.two = two;
+  turns.two = two ? 1 : 0;
   turns.t_begin = int(int64_t(split) * t.chunks / a.splits);
   turns.t_end = int(int64_t(split + 1) * t.chunks / a.splits);
-  for (int s = 0; s < 2; ++s) {
-    turns.sinks[s] = turns.begin[s] = 0;
-    turns.end[s] = t.chunks;
-    if (!two || a.depth != nullptr) continue;
+  turns.sinks0 = turns.begin0 = turns.sinks1 = turns.begin1 = 0;
+  turns.end0 = turns.end1 = t.chunks;
+  if (two && a.depth == nullptr) {
     const int mid = u->i0 + kTile;
-    const TileKeys k = s == 0 ? causal_keys(a, u->r, j0, (mid - 1) / a.group) : causal_keys(a, u->r, mid / a.group, j1);
-    u->stream_keys[s] = k;
     const int main = t.sink_chunks - t.lo / kTile;  // from a key's tile to its number
-    turns.sinks[s] = min(t.sink_chunks, (k.sinks + kTile - 1) / kTile);
-    turns.begin[s] = k.sinks > t.lo / kTile * kTile ? t.sink_chunks : main + k.lo / kTile;
-    turns.end[s] = main + (k.end + kTile - 1) / kTile;
+    auto limit = [&](const TileKeys& k, int& sinks, int& begin, int& end) {
+      sinks = min(t.sink_chunks, (k.sinks + kTile - 1) / kTile);
+      begin = k.sinks > t.lo / kTile * kTile ? t.sink_chunks : main + k.lo / kTile;
+      end = main + (k.end + kTile - 1) / kTile;
+    };
+    u->stream_keys[0] = causal_keys(a, u->r, j0, (mid - 1) / a.group);
+    u->stream_keys[1] = causal_keys(a, u->r, mid / a.group, j1);
+    limit(u->stream_keys[0], turns.sinks0, turns.begin0, turns.end0);
+    limit(u->stream_keys[1], turns.sinks1, turns.begin1, turns.end1);
   }
   return true;
 }
@@ -277,159 +281,229 @@ struct TileScales {
   float k[kTile], log_v[kTile], inv_v[kTile];  // by key; where `one`, the first of each is the tile's
 };
 
-// What fetching threads share of a tile (in turns of two).
+// What the fetching threads share of a tile.
 struct FetchRows {
-  uint32_t row[2][kTile];
-  float scale[2][kTile];   // e4m3: the largest scale's share that the key's is, or 1 for all
-  float low[4], high[4];   // by warp
-  int odd[4];
-  int abort;               // a wait ran out: the four warps stop together
+  uint32_t row[2][kTile];                            // of a tile's keys, in turns of two
+  float k_relative[2][kTile], v_relative[2][kTile];  // e4m3: the share of the tile's largest scale that a key's is, or 1
+  float low[2][4], high[2][4];                       // K's and V's, by warp
+  int odd[2][4];
+  int abort;                                         // a wait ran out: the four warps stop together
 };
-static_assert(sizeof(TileScales) == 3 * kTile * 4 && sizeof(FetchRows) <= 2176, "shared memory");
+static_assert(sizeof(TileScales) == 3 * kTile * 4 && sizeof(FetchRows) <= kFetchBytes, "shared memory");
 
-// The scale of a key of e4m3 codes, relative to the tile's largest; whether the tile has one scale. 128 threads, a key
-// each (`live` false: none), `named` their barrier.
-__device__ __forceinline__ bool one_scale(FetchRows* rows, int named, bool live, float scale, float* relative, float* top) {
-  const int tid = threadIdx.x & (kRoleThreads - 1), warp = tid >> 5;
+// Of the scales of a tile's keys, a key each thread (`live` false: none), what one warp sees of them.
+__device__ __forceinline__ void note_scales(FetchRows* rows, int which, bool live, float scale) {
+  const int tid = threadIdx.x & (kRoleThreads - 1);
   const float low = -warp_max(live ? -scale : -INFINITY), high = warp_max(live ? scale : 0.f);
-  const uint32_t bits = __float_as_uint(scale);
-  const bool odd = __any_sync(0xffffffffu, live && ((bits & 0x7fffffu) != 0 || !(scale > 0.f && scale < INFINITY)));
+  const bool odd = __any_sync(0xffffffffu, live && ((__float_as_uint(scale) & 0x7fffffu) != 0 ||
+                                                    !(scale > 0.f && scale < INFINITY)));
   if ((tid & 31) == 0) {
-    rows->low[warp] = low;
-    rows->high[warp] = high;
-    rows->odd[warp] = odd ? 1 : 0;
+    rows->low[which][tid >> 5] = low;
+    rows->high[which][tid >> 5] = high;
+    rows->odd[which][tid >> 5] = odd ? 1 : 0;
   }
-  named_barrier_sync(named, kRoleThreads);
-  const float least = fminf(fminf(rows->low[0], rows->low[1]), fminf(rows->low[2], rows->low[3]));
-  *top = fmaxf(fmaxf(rows->high[0], rows->high[1]), fmaxf(rows->high[2], rows->high[3]));
-  const bool one = (rows->odd[0] | rows->odd[1] | rows->odd[2] | rows->odd[3]) == 0 && *top > 0.f && least * 32768.f >= *top;
+}
+// Whether the tile has one scale, after a barrier; *top is the largest, *relative the share of it that `scale` is.
+__device__ __forceinline__ bool one_scale(const FetchRows* rows, int which, bool live, float scale, float* relative,
+                                          float* top) {
+  const float* low = rows->low[which];
+  const float* high = rows->high[which];
+  const int* odd = rows->odd[which];
+  *top = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3]));
+  const bool one = (odd[0] | odd[1] | odd[2] | odd[3]) == 0 && *top > 0.f &&
+                   fminf(fminf(low[0], low[1]), fminf(low[2], low[3])) * 32768.f >= *top;
   // the quotient of two powers of two
-  *relative = one && live ? __uint_as_float(bits - __float_as_uint(*top) + 0x3f800000u) : 1.f;
+  *relative = one && live ? __uint_as_float(__float_as_uint(scale) - __float_as_uint(*top) + 0x3f800000u) : 1.f;
   return one;
 }
 
-// Fetches all key tiles (VALUES false) or value tiles of the CTA into its ring of two: 128 threads.
-template <int HD, typename T, bool E4M3, bool VALUES>
+// Fetches all key and value tiles of the CTA into their rings of two: 128 threads.
+template <int HD, typename T, bool E4M3>
 __device__ __forceinline__ void fetch_tiles(const CacheAttnArgs& a, const Unit& u, uint8_t* smem, PrefillBarriers* bars) {
   using S = PrefillSmem<HD>;
+  constexpr int NAMED = 2;
   const int tid = threadIdx.x & (kRoleThreads - 1), lane = tid & 31;
-  constexpr int NAMED = VALUES ? 3 : 2;
-  uint64_t* full = VALUES ? bars->v_full : bars->k_full;
-  uint64_t* empty = VALUES ? bars->v_empty : bars->k_empty;
-  uint8_t* ring = smem + (VALUES ? S::V : S::K);
-  FetchRows* share = reinterpret_cast<FetchRows*>(smem + S::FETCH) + (VALUES ? 1 : 0);
-  const uint8_t* plane = static_cast<const uint8_t*>(VALUES ? a.c.v : a.c.k);
+  FetchRows* share = reinterpret_cast<FetchRows*>(smem + S::FETCH);
   constexpr int ES = E4M3 ? 1 : 2;
   constexpr int VECS = HD * ES / 16;            // 16-byte vectors of a row in the page
   constexpr int PER_PASS = kRoleThreads / VECS; // rows that the threads fetch together
   constexpr int PASSES = kTile / PER_PASS;
   const int vec = tid % VECS, first = tid / VECS;
+  const uint8_t* const k_plane = static_cast<const uint8_t*>(a.c.k) + vec * 16;
+  const uint8_t* const v_plane = static_cast<const uint8_t*>(a.c.v) + vec * 16;
   const PageRows rows = {a.s.tables + u.seq * a.s.table_stride, a.c.page_shift, a.c.page_size - 1,
                          a.c.num_pages, a.c.kv_heads, u.head, a.err};
   const TileKeys keys = u.keys;
   const int t_begin = u.turns.t_begin, tiles = u.turns.t_end - t_begin;
-  uint32_t next = tiles > 0 ? rows.row(keys, keys.key<kTile>(t_begin) + tid) : kNoRow;
-  for (int n = 0; n < tiles; ++n) {
-    const int kv0 = keys.key<kTile>(t_begin + n);
-    // the rows of this tile's keys for all threads, the next tile's on their way
-    const uint32_t mine = next;
-    share->row[n & 1][tid] = mine;
-    if (n + 1 < tiles) next = rows.row(keys, keys.key<kTile>(t_begin + n + 1) + tid);
-    const bool look = VALUES && !keys.all_seen(kv0, kTile);  // for values that are no numbers
-    uint8_t* dst = ring + (n & 1) * S::TILE;
-    if constexpr (!E4M3) {
-      if (n >= 2 && !warp_wait(empty + (n & 1), ((n >> 1) - 1) & 1, a.err, kErrTimeoutEmpty)) share->abort = 1;
-      named_barrier_sync(NAMED, kRoleThreads);
-      if (share->abort) break;
+  auto arrive = [&](uint64_t* bar) {
+    fence_proxy_async_shared();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
+  };
+  // A tile's place in a ring, free: false (for all four warps) once a wait has run out.
+  auto place = [&](uint64_t* empty, int n) {
+    if (n < 2) return true;
+    if (!warp_wait(empty + (n & 1), ((n >> 1) - 1) & 1, a.err, kErrTimeoutEmpty)) share->abort = 1;
+    named_barrier_sync(NAMED, kRoleThreads);
+    return share->abort == 0;
+  };
+  auto row_of = [&](int n) { return n < tiles ? rows.row(keys, keys.key<kTile>(t_begin + n) + tid) : kNoRow; };
+  auto masked = [&](int n) { return !keys.all_seen(keys.key<kTile>(t_begin + n), kTile); };  // not every row sees every key
+  if constexpr (!E4M3) {
+    // In turns the copies of K(n) and V(n - 1), and of V(n) and K(n), are on their way together. What a place waits for
+    // needs no tile that has not been announced: K(n)'s place the products Q K(n - 2), V(n)'s the products P V(n - 2).
+    uint32_t next = row_of(0);
+    auto copy = [&](uint8_t* dst, const uint8_t* plane, int n) {
+      const uint32_t* const row = share->row[n & 1];
 #pragma unroll
       for (int p = 0; p < PASSES; ++p) {
-        const uint32_t from = share->row[n & 1][first + p * PER_PASS];
-        cp_async_16(dst + tile_at(first + p * PER_PASS, vec),
-                    plane + (from == kNoRow ? 0 : size_t(from) * (HD * ES) + vec * 16), from != kNoRow);
+        const uint32_t from = row[first + p * PER_PASS];
+        cp_async_16(dst + (n & 1) * S::TILE + tile_at(first + p * PER_PASS, vec),
+                    plane + (from == kNoRow ? 0 : size_t(from) * (HD * ES)), from != kNoRow);
       }
       cp_async_commit();
-      cp_async_wait<0>();
-      if (look) {
+    };
+    auto values_landed = [&](int n) {
+      if (masked(n)) {
 #pragma unroll 1
         for (int p = 0; p < PASSES; ++p) {
-          uint4* x = reinterpret_cast<uint4*>(dst + tile_at(first + p * PER_PASS, vec));
+          uint4* x = reinterpret_cast<uint4*>(smem + S::V + (n & 1) * S::TILE + tile_at(first + p * PER_PASS, vec));
           if (any_non_finite<T, false>(*x)) {
             drop_non_finite<T, false>(*x);
             bars->odd = 1;
           }
         }
       }
-    } else {
-      const uint32_t block = mine == kNoRow ? 0 : mine >> a.c.block_shift;  // blocks divide pages: their numbers run on
-      const bool live = mine != kNoRow;
-      const float vs = live ? fmaxf(a.c.v_scale[block], kLeastScale) : 1.f;
-      float relative, v_top;
-      const bool v_one = one_scale(share, NAMED, live, vs, &relative, &v_top);
-      bool in_time = true;
-      if constexpr (!VALUES) {
-        const float ks = live ? a.c.k_scale[block] : 1.f;
-        float k_top;
-        named_barrier_sync(NAMED, kRoleThreads);
-        const bool k_one = one_scale(share, NAMED, live, ks, &relative, &k_top);
-        in_time = n < 2 || warp_wait(empty + (n & 1), ((n >> 1) - 1) & 1, a.err, kErrTimeoutEmpty);
-        if (in_time) {
-          // The scales' slot: its last readers, the softmax of tile n - 4, are done. The products Q K of tiles n - 3 and
-          // n - 2 have run, and a stream's products start only when its softmax of the tile before is over.
-          const int slot = n % kScaleSlots;
-          TileScales& scales = reinterpret_cast<TileScales*>(smem + S::SCALES)[slot];
-          const float v = v_one ? v_top : vs;
-          scales.k[tid] = k_one ? k_top : ks;
-          scales.log_v[tid] = lg2(v);
-          scales.inv_v[tid] = rcp(v);
-          if (tid == 0) bars->one[slot] = k_one && v_one ? 1 : 0;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bars->scales_full + slot);
-        }
-      } else {
-        in_time = n < 2 || warp_wait(empty + (n & 1), ((n >> 1) - 1) & 1, a.err, kErrTimeoutEmpty);
-      }
-      if (!in_time) share->abort = 1;
-      share->scale[n & 1][tid] = relative;
+      arrive(bars->v_full + (n & 1));
+    };
+    int n = 0;
+    for (; n < tiles; ++n) {
+      share->row[n & 1][tid] = next;
+      next = row_of(n + 1);
       named_barrier_sync(NAMED, kRoleThreads);
-      if (share->abort) break;
-      constexpr int HELD = 4;  // vectors of codes a thread has on their way at once
-#pragma unroll 1
-      for (int p0 = 0; p0 < PASSES; p0 += HELD) {
-        uint4 codes[HELD];
+      if (!place(bars->k_empty, n)) break;
+      copy(smem + S::K, k_plane, n);
+      if (n > 0) {
+        cp_async_wait<1>();
+        values_landed(n - 1);
+      }
+      if (!place(bars->v_empty, n)) break;
+      copy(smem + S::V, v_plane, n);
+      cp_async_wait<1>();
+      arrive(bars->k_full + (n & 1));
+    }
+    cp_async_wait<0>();
+    if (n == tiles && tiles > 0) values_landed(tiles - 1);
+  } else {
+    // A tile's codes are on their way to registers while the tile before is stored.
+    auto load = [&](uint4(&codes)[PASSES], const uint8_t* plane, int n) {
+      const uint32_t* const row = share->row[n & 1];
 #pragma unroll
-        for (int p = 0; p < HELD; ++p) {
-          const uint32_t from = share->row[n & 1][first + (p0 + p) * PER_PASS];
-          codes[p] = make_uint4(0, 0, 0, 0);
-          if (from != kNoRow) codes[p] = *reinterpret_cast<const uint4*>(plane + size_t(from) * HD + vec * 16);
+      for (int p = 0; p < PASSES; ++p) {
+        const uint32_t from = row[first + p * PER_PASS];
+        codes[p] = make_uint4(0, 0, 0, 0);
+        if (from != kNoRow) codes[p] = *reinterpret_cast<const uint4*>(plane + size_t(from) * HD);
+      }
+    };
+    // 16 codes of a row to f16 times the row's share of the tile's scale, exactly.
+    auto store = [&](uint8_t* dst, const uint4(&codes)[PASSES], const float* relative) {
+#pragma unroll
+      for (int p = 0; p < PASSES; ++p) {
+        const int at = first + p * PER_PASS;
+        const __half2 by = __float2half2_rn(relative[at]);
+        const uint32_t w[4] = {codes[p].x, codes[p].y, codes[p].z, codes[p].w};
+        uint32_t h[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t x = e4m3x2_to_f16x2(uint16_t(w[i / 2] >> (16 * (i & 1))));
+          const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&x), by);
+          h[i] = *reinterpret_cast<const uint32_t*>(&y);
         }
+        // the upper half of a row's threads the other way round: all eight groups of banks in each store
+        const uint4 x = make_uint4(h[0], h[1], h[2], h[3]), y = make_uint4(h[4], h[5], h[6], h[7]);
+        const bool swap = HD == 128 && vec >= 4;
+        *reinterpret_cast<uint4*>(dst + tile_at(at, 2 * vec + (swap ? 1 : 0))) = swap ? y : x;
+        *reinterpret_cast<uint4*>(dst + tile_at(at, 2 * vec + (swap ? 0 : 1))) = swap ? x : y;
+      }
+    };
+    auto block_of = [&](uint32_t row) { return row == kNoRow ? 0 : row >> a.c.block_shift; };  // blocks divide pages
+    uint4 k_codes[PASSES], v_codes[PASSES];
+    uint32_t mine = row_of(0), next = row_of(1);
+    float ks = a.c.k_scale[block_of(mine)], vs = a.c.v_scale[block_of(mine)];
+    share->row[0][tid] = mine;
+    named_barrier_sync(NAMED, kRoleThreads);
+    if (tiles > 0) {
+      load(k_codes, k_plane, 0);
+      load(v_codes, v_plane, 0);
+    }
+    for (int n = 0; n < tiles; ++n) {
+      const bool live = mine != kNoRow;
+      if (!live) ks = vs = 1.f;
+      vs = fmaxf(vs, kLeastScale);
+      share->row[(n + 1) & 1][tid] = next;
+      note_scales(share, 0, live, ks);
+      note_scales(share, 1, live, vs);
+      named_barrier_sync(NAMED, kRoleThreads);
+      float k_relative, v_relative, k_top, v_top;
+      const bool k_one = one_scale(share, 0, live, ks, &k_relative, &k_top);
+      const bool v_one = one_scale(share, 1, live, vs, &v_relative, &v_top);
+      share->k_relative[n & 1][tid] = k_relative;
+      share->v_relative[n & 1][tid] = v_relative;
+      mine = next;
+      const float ks_next = a.c.k_scale[block_of(mine)], vs_next = a.c.v_scale[block_of(mine)];
+      next = row_of(n + 2);
+      if (!place(bars->k_empty, n)) break;
+      {
+        // The scales' slot: its last readers, the softmax of tile n - 4, are done. The products Q K of tiles n - 3 and
+        // n - 2 have run, and a stream's products start only when its softmax of the tile before is over.
+        const int slot = n % kScaleSlots;
+        TileScales& scales = reinterpret_cast<TileScales*>(smem + S::SCALES)[slot];
+        const float v = v_one ? v_top : vs;
+        scales.k[tid] = k_one ? k_top : ks;
+        scales.log_v[tid] = lg2(v);
+        scales.inv_v[tid] = rcp(v);
+        if (tid == 0) bars->one[slot] = k_one && v_one ? 1 : 0;
+        named_barrier_sync(NAMED, kRoleThreads);  // and every key's share of the scale is there
+        if (lane == 0) mbar_arrive(bars->scales_full + slot);
+      }
+      ks = ks_next;
+      vs = vs_next;
+      store(smem + S::K + (n & 1) * S::TILE, k_codes, share->k_relative[n & 1]);
+      arrive(bars->k_full + (n & 1));
+      load(k_codes, k_plane, n + 1);
+      if (masked(n)) {
 #pragma unroll
-        for (int p = 0; p < HELD; ++p) {
-          if (look && any_non_finite<T, true>(codes[p])) {
-            drop_non_finite<T, true>(codes[p]);
+        for (int p = 0; p < PASSES; ++p) {
+          if (any_non_finite<T, true>(v_codes[p])) {
+            drop_non_finite<T, true>(v_codes[p]);
             bars->odd = 1;
           }
-          const int row = first + (p0 + p) * PER_PASS;
-          const __half2 by = __float2half2_rn(share->scale[n & 1][row]);
-          const uint32_t w[4] = {codes[p].x, codes[p].y, codes[p].z, codes[p].w};
-          uint32_t h[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const uint32_t x = e4m3x2_to_f16x2(uint16_t(w[i / 2] >> (16 * (i & 1))));
-            const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&x), by);
-            h[i] = *reinterpret_cast<const uint32_t*>(&y);
-          }
-          *reinterpret_cast<uint4*>(dst + tile_at(row, 2 * vec)) = make_uint4(h[0], h[1], h[2], h[3]);
-          *reinterpret_cast<uint4*>(dst + tile_at(row, 2 * vec + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
         }
       }
+      if (!place(bars->v_empty, n)) break;
+      store(smem + S::V + (n & 1) * S::TILE, v_codes, share->v_relative[n & 1]);
+      arrive(bars->v_full + (n & 1));
+      load(v_codes, v_plane, n + 1);
     }
-    fence_proxy_async_shared();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(full + (n & 1));
   }
 }
 
-// Issues all products: one thread, so that nothing of its warp has to be brought together again after a wait.
+// Whether a barrier's phase is complete, at once (mbar_try_wait may hold the thread for a while).
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// Issues all products: one thread, so that nothing of its warp has to be brought together again after a wait. It looks
+// at the streams in turn and issues P V and the next Q K of the one whose softmax is over, together: two streams whose
+// products mixed would finish, and start their softmax, at the same time.
 template <int HD, bool BF16>
 __device__ __forceinline__ void issue_products(const CacheAttnArgs& a, const Turns& turns, uint8_t* smem,
                                                PrefillBarriers* bars) {
@@ -441,59 +515,83 @@ __device__ __forceinline__ void issue_products(const CacheAttnArgs& a, const Tur
   const uint32_t tmem = bars->tmem;
   const uint64_t q_desc = umma_desc_sw128(smem_u32(smem + S::Q)), k_desc = umma_desc_sw128(smem_u32(smem + S::K));
   const uint64_t v_desc = umma_desc_transposed(smem_u32(smem + S::V), PANEL);
-  const bool two = turns.two;
   const int t_begin = turns.t_begin, tiles = turns.t_end - t_begin;
-  bool ok = true;
-  auto wait = [&](uint64_t* bar, uint32_t parity, int code) { ok = ok && mbar_wait(bar, parity, a.err, code); };
   auto scores = [&](int s, int n) {
-    wait(bars->k_full + (n & 1), (n >> 1) & 1, kErrTimeoutFull);
-    if (!ok) return;
-    tc_fence_after();
-    const uint64_t q = q_desc + (two ? s * STEP : 0), k = k_desc + (n & 1) * STEP;
+    const uint64_t q = q_desc + (turns.two ? s * STEP : 0), k = k_desc + (n & 1) * STEP;
+    const uint32_t d = tmem + s * kTile;
 #pragma unroll
     for (int x = 0; x < HD / 16; ++x) {
       const int at = ((x >> 2) * PANEL + (x & 3) * 32) >> 4;
-      umma_f16(tmem + s * kTile, q + at, k + at, QK, x > 0 ? 1u : 0u);
+      umma_f16(d, q + at, k + at, QK, x > 0 ? 1u : 0u);
     }
     umma_commit(bars->s_full + s);
     umma_commit(bars->k_empty + (n & 1));
     if (!turns.active(1 - s, t_begin + n)) umma_commit(bars->k_empty + (n & 1));  // the other stream has no use for it
   };
-  auto values = [&](int s, int n, int count) {
-    wait(bars->v_full + (n & 1), (n >> 1) & 1, kErrTimeoutFull);
-    wait(bars->p_ready + s, count & 1, kErrTimeoutPeer);
-    if (!ok) return;
-    tc_fence_after();
-    const uint64_t v = v_desc + (n & 1) * STEP;
-#pragma unroll
-    for (int x = 0; x < kTile / 16; ++x)
-      umma_f16_ts(tmem + 2 * kTile + s * kTile, tmem + s * kTile + x * 8, v + ((x * 2048) >> 4), PV,
-                  count > 0 || x > 0 ? 1u : 0u);
-    umma_commit(bars->pv_done + s);
-    umma_commit(bars->v_empty + (n & 1));
-    if (!turns.active(1 - s, t_begin + n)) umma_commit(bars->v_empty + (n & 1));
+  if (!mbar_wait(&bars->q_ready, 0, a.err, kErrTimeoutPeer)) return;
+  // The stream looked at and the other one: its tile, that tile's number among the stream's, and whether its scores have
+  // been asked for (then the product with the values is next). Nothing is waited for here: a stream that is ahead may need
+  // a tile whose place the other one has yet to free.
+  struct State {
+    int n, count;
+    bool scored;
   };
-  auto after = [&](int s, int n) {  // the stream's next tile from n on
-    while (n < tiles && !turns.active(s, t_begin + n)) ++n;
-    return n;
-  };
-  wait(&bars->q_ready, 0, kErrTimeoutPeer);
-  int at[2] = {after(0, 0), after(1, 0)}, count = 0;
+  State now = {turns.next(0, t_begin) - t_begin, 0, false}, other = {turns.next(1, t_begin) - t_begin, 0, false};
+  int s = 0;
+  uint64_t since = 0;
+  uint32_t looks = 0;  // the timer takes longer to read than everything else here
+  while (now.n < tiles || other.n < tiles) {
+    ++looks;
+    if (now.n < tiles && now.scored && mbar_test(bars->p_ready + s, now.count & 1) &&
+        mbar_test(bars->v_full + (now.n & 1), (now.n >> 1) & 1)) {
+      tc_fence_after();
+      const uint64_t v = v_desc + (now.n & 1) * STEP;
+      const uint32_t p = tmem + s * kTile;
 #pragma unroll
-  for (int s = 0; s < 2; ++s)
-    if (at[s] < tiles) scores(s, at[s]);
-  while (ok && (at[0] < tiles || at[1] < tiles)) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      if (at[s] >= tiles) continue;
-      const int next = after(s, at[s] + 1);
-      values(s, at[s], count);
-      if (next < tiles) scores(s, next);
-      at[s] = next;
+      for (int x = 0; x < kTile / 16; ++x)
+        umma_f16_ts(p + 2 * kTile, p + x * 8, v + ((x * 2048) >> 4), PV, now.count > 0 || x > 0 ? 1u : 0u);
+      umma_commit(bars->pv_done + s);
+      umma_commit(bars->v_empty + (now.n & 1));
+      if (!turns.active(1 - s, t_begin + now.n)) umma_commit(bars->v_empty + (now.n & 1));
+      now = {turns.next(s, t_begin + now.n + 1) - t_begin, now.count + 1, false};
+      looks = 0;
     }
-    ++count;
+    if (now.n < tiles && !now.scored && mbar_test(bars->k_full + (now.n & 1), (now.n >> 1) & 1)) {
+      tc_fence_after();
+      scores(s, now.n);
+      now.scored = true;
+      looks = 0;
+    }
+    if (looks >= 4096 && (looks & 4095) == 0) {
+      if (looks == 4096) since = global_timer_ns();
+      if (global_timer_ns() - since > kWaitLimitNs) {
+        record_error(a.err, kErrTimeoutPeer);
+        return;
+      }
+    }
+    const State x = now;
+    now = other;
+    other = x;
+    s ^= 1;
   }
 }
+
+// A thread's packed rows when the threads of a stream go through its tile together, every N-th: as row of the sequence
+// and head of the group.
+template <int N>
+struct RowWalk {
+  static constexpr int STEP = N;
+  int packed, j, g, dj, dg;
+  __device__ __forceinline__ void advance(int group) {
+    packed += N;
+    j += dj;
+    g += dg;
+    if (g >= group) {
+      g -= group;
+      ++j;
+    }
+  }
+};
 
 template <int HD, typename T, bool E4M3>
 __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(const CacheAttnArgs a) {
@@ -526,7 +624,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
     }
     for (int i = 0; i < kScaleSlots; ++i) mbar_init(bars->scales_full + i, 4);
     bars->odd = 0;
-    for (int i = 0; i < 2; ++i) reinterpret_cast<FetchRows*>(smem + S::FETCH)[i].abort = 0;
+    reinterpret_cast<FetchRows*>(smem + S::FETCH)->abort = 0;
     fence_barrier_init();
   }
   __syncthreads();
@@ -540,22 +638,15 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
   tc_fence_after();
   const uint32_t tmem = bars->tmem;
 
-  // Registers: 96 a thread at launch, 5 x 96 = 480 for the five groups of four warps: 2 x 168 + 2 x 48 + 48 = 480.
   const int role = tid / kRoleThreads;
   if (role == 2) {
-    registers_dec<48>();
-    fetch_tiles<HD, T, E4M3, false>(a, u, smem, bars);
+    fetch_tiles<HD, T, E4M3>(a, u, smem, bars);
   } else if (role == 3) {
-    registers_dec<48>();
-    fetch_tiles<HD, T, E4M3, true>(a, u, smem, bars);
-  } else if (role == 4) {
-    registers_dec<48>();
-    if (tid == 4 * kRoleThreads) {
+    if (lane == 0) {
       const Turns turns = u.turns;
       issue_products<HD, std::is_same<M, __nv_bfloat16>::value>(a, turns, smem, bars);
     }
   } else {
-    registers_inc<168>();
     const int stream = role;
     float m = -INFINITY, l = 0.f;
     int done = 0;  // key tiles this stream has worked on
@@ -564,49 +655,67 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
     const int row = tid & (kRoleThreads - 1);                       // of the stream's tile
     const int i = u.i0 + (u.turns.two && stream == 1 ? kTile : 0) + row;  // packed row
     const bool live = i < u.i0 + u.rows;
-    // ---- the row's query into shared memory (with one row tile, stream 0's threads bring it)
+    // ---- the stream's queries into shared memory (with one row tile both streams' are the same, and stream 0 brings
+    // them): 16-byte vectors along the rows, then each row to f16 by its own thread where that has to be
+    constexpr bool RESCALE = E4M3 && std::is_same<T, __nv_bfloat16>::value;
+    constexpr int QV = HD / 8;  // vectors of a row
+    using Walk = RowWalk<kRoleThreads / QV>;
+    const int walk_first = i - row + row / QV;
+    const Walk walk = {walk_first, walk_first / a.group, walk_first % a.group, Walk::STEP / a.group, Walk::STEP % a.group};
+    uint8_t* const q_tile = smem + S::Q + (u.turns.two ? stream : 0) * S::TILE;
+    const int unit_rows = u.i0 + u.rows;
+    if (u.turns.two || stream == 0) {
+      Walk at = walk;
+#pragma unroll
+      for (int p = 0; p < QV; ++p, at.advance(a.group)) {
+        const bool there = at.packed < unit_rows;
+        const T* from = static_cast<const T*>(a.q) + (u.r.start + at.j) * a.q_stride + (u.head * a.group + at.g) * HD;
+        cp_async_16(q_tile + tile_at(row / QV + p * Walk::STEP, row % QV),
+                    there ? from + row % QV * 8 : static_cast<const T*>(a.q), there);
+      }
+      cp_async_commit();
+      cp_async_wait<0>();
+    }
     float q_scale = a.scale_log2;
-    const T* src = static_cast<const T*>(a.q) + (u.r.start + (live ? i : u.i0) / a.group) * a.q_stride +
-                   (u.head * a.group + (live ? i : u.i0) % a.group) * HD;
-    float up = 1.f;
-    if constexpr (E4M3 && std::is_same<T, __nv_bfloat16>::value) {
+    if constexpr (RESCALE) {
+      named_barrier_sync(1, 2 * kRoleThreads);  // both streams read the rows, one may write them
       uint32_t top = 0;
-#pragma unroll 4
-      for (int vec = 0; vec < HD / 8; ++vec) {
-        const uint4 x = live ? reinterpret_cast<const uint4*>(src)[vec] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int vec = 0; vec < QV; ++vec) {
+        const uint4 x = *reinterpret_cast<const uint4*>(q_tile + tile_at(row, vec));
         const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) top = max(top, max(w[e] & 0x7fffu, (w[e] >> 16) & 0x7fffu));
       }
       const int e = query_exponent(top);
-      up = power_of_two_f32(-e);
+      const float up = power_of_two_f32(-e);
       q_scale *= power_of_two_f32(e);
-    }
-    if (u.turns.two || stream == 0) {
-      uint8_t* dst = smem + S::Q + stream * S::TILE;
-#pragma unroll 4
-      for (int vec = 0; vec < HD / 8; ++vec) {
-        uint4 x = live ? reinterpret_cast<const uint4*>(src)[vec] : make_uint4(0, 0, 0, 0);
-        if constexpr (E4M3 && std::is_same<T, __nv_bfloat16>::value) {
-          uint32_t* w = &x.x;
+      named_barrier_sync(1, 2 * kRoleThreads);
+      if (u.turns.two || stream == 0) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            w[e] = pack2<__half>(__uint_as_float(w[e] << 16) * up, __uint_as_float(w[e] & 0xffff0000u) * up);
+        for (int vec = 0; vec < QV; ++vec) {
+          uint4* at = reinterpret_cast<uint4*>(q_tile + tile_at(row, vec));
+          const uint4 x = *at;
+          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+          uint32_t h[4];
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            h[y] = pack2<__half>(__uint_as_float(w[y] << 16) * up, __uint_as_float(w[y] & 0xffff0000u) * up);
+          *at = make_uint4(h[0], h[1], h[2], h[3]);
         }
-        *reinterpret_cast<uint4*>(dst + tile_at(row, vec)) = x;
       }
     }
     fence_proxy_async_shared();
     __syncwarp();
     if (lane == 0) mbar_arrive(&bars->q_ready);
-    const RowMask mask = live ? row_mask(a, u.r, i / a.group) : no_row();
+    auto row_sees = [&]() { return live ? row_mask(a, u.r, i / a.group) : no_row(); };
     const Turns turns = u.turns;
     const int full_lo = u.stream_keys[stream].full_lo, full_end = u.stream_keys[stream].full_end,
               full_sinks = u.stream_keys[stream].sinks;
     const uint32_t t_s = t_lane + stream * kTile, t_o = t_lane + 2 * kTile + stream * kTile;
 
-    for (int n = 0; n < turns.t_end - turns.t_begin; ++n) {
-      if (!turns.active(stream, turns.t_begin + n)) continue;
+    for (int n = turns.next(stream, turns.t_begin) - turns.t_begin; n < turns.t_end - turns.t_begin;
+         n = turns.next(stream, turns.t_begin + n + 1) - turns.t_begin) {
       const int kv0 = u.keys.key<kTile>(turns.t_begin + n);
       const bool full = kv0 + kTile <= full_end && (kv0 >= full_lo || kv0 + kTile <= full_sinks);
       const int slot = n % kScaleSlots;
@@ -624,26 +733,21 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
         inv_v = scales.inv_v[0];
       }
       by = fmaxf(by, 1.17549435e-38f);
-      auto hide = [&](int c, float* x, int count) {  // scores of keys c.. of the tile that the row does not see
-        const int last = mask.last - kv0 - c, first = mask.first - kv0 - c, sinks = a.sinks - kv0 - c;
-        if (a.depth == nullptr) {
-#pragma unroll
-          for (int e = 0; e < count; ++e)
-            if (!((e <= last) & ((e >= first) | (e < sinks)))) x[e] = -INFINITY;
-        } else {
-          const int own_first = mask.own_first - kv0 - c, own_last = mask.own_last - kv0 - c;
-#pragma unroll
-          for (int e = 0; e < count; ++e)
-            if (!(((e <= last) & ((e >= first) | (e < sinks))) | ((e >= own_first) & (e <= own_last)))) x[e] = -INFINITY;
-        }
+      // Bit e: whether the row sees key c + e of the tile, 32 of them.
+      auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };  // bits [0, n)
+      RowMask mask = no_row();
+      if (!full) mask = row_sees();
+      auto seen = [&](int c) {
+        const int at = kv0 + c;
+        uint32_t bits = below(mask.last + 1 - at) & (~below(mask.first - at) | below(a.sinks - at));
+        if (a.depth != nullptr) bits |= below(mask.own_last + 1 - at) & ~below(mask.own_first - at);
+        return bits;
       };
-      auto largest = [&](const float* x, int count) {
-        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      auto hide = [&](int c, float* x) {
+        const uint32_t bits = seen(c);
 #pragma unroll
-        for (int e = 0; e < count; e += 8)
-#pragma unroll
-          for (int y = 0; y < 4; ++y) tops[y] = fmaxf(fmaxf(tops[y], x[e + 2 * y]), x[e + 2 * y + 1]);
-        return fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+        for (int e = 0; e < 32; ++e)
+          if (!(bits & (1u << e))) x[e] = -INFINITY;
       };
       // A row's maximum to `top` (in units of log2), O and l with it.
       auto raise = [&](float top) {
@@ -658,36 +762,21 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
 #pragma unroll 1
         for (int c = 0; c < HD; c += 16) {
           float y[16];
-          tmem_ld_16cols(t_o + c, y);
+          tmem_ld_16(t_o + c, y);
+          tmem_wait_ld();
           uint32_t z[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) z[e] = __float_as_uint(y[e] * keep);
           tmem_st_16cols(t_o + c, z);
         }
       };
-      // The tile's maxima alone: the first tile's, and those of a tile with many scales.
-      auto tile_maximum = [&]() {
-        float top = -INFINITY;
-#pragma unroll 1
-        for (int c = 0; c < kTile; c += 16) {
-          float x[16];
-          tmem_ld_16cols(t_s + c, x);
-          if (!full) hide(c, x, 16);
-          if (one) {
-            top = fmaxf(top, largest(x, 16));
-          } else {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) top = fmaxf(top, fmaf(x[e] * by, scales.k[c + e], scales.log_v[c + e]));
-          }
-        }
-        return !one || top == -INFINITY ? top : fmaf(top, by, add);
-      };
       if (one) {
-        if (done == 0) raise(tile_maximum());
-        // One pass with the maximum as it is; should it prove too small, it is raised and the pass repeated.
+        // One pass with the maximum as it is, 0 for a row that has seen no key yet; should it prove too small, or the
+        // guess too large, it is put right and the pass repeated.
         uint32_t p[kTile / 2];
         while (true) {
-          const float from = add - (m == -INFINITY ? 0.f : m);
+          const bool fresh = m == -INFINITY;
+          const float from = add - (fresh ? 0.f : m);
           const f32x2 scale2 = pair(by, by), from2 = pair(from, from);
           f32x2 sums[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
           float top = -INFINITY;
@@ -698,8 +787,14 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
             float(&y)[32] = x[(c / 32) & 1];
             tmem_wait_ld();
             if (c + 32 < kTile) tmem_ld_32(t_s + c + 32, x[(c / 32 + 1) & 1]);
-            if (!full) hide(c, y, 32);
-            top = fmaxf(top, largest(y, 32));
+            if (!full) hide(c, y);
+            float tops[2] = {top, -INFINITY};
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              tops[0] = fmaxf(fmaxf(tops[0], y[e]), y[e + 1]);
+              tops[1] = fmaxf(fmaxf(tops[1], y[e + 2]), y[e + 3]);
+            }
+            top = fmaxf(tops[0], tops[1]);
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
               float lo, hi;
@@ -711,10 +806,12 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
             }
           }
           top = top == -INFINITY ? top : fmaf(top, by, add);
-          if (!__any_sync(0xffffffffu, top > m + kLazy)) {
+          const bool again = fresh ? top > kLazy || (top < -kGuess && top > -INFINITY) : top > m + kLazy;
+          if (!__any_sync(0xffffffffu, again)) {
             float lo, hi;
             unpair(add2(sums[0], sums[1]), lo, hi);
             l = fmaf(lo + hi, inv_v, l);
+            if (fresh && top > -INFINITY) m = 0.f;
             break;
           }
           raise(top);
@@ -724,7 +821,16 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_st_16cols(t_s + c * 16, p + c * 16);  // over scores that have been read
       } else {
-        const float top = tile_maximum();
+        float top = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < kTile; c += 32) {
+          float x[32];
+          tmem_ld_32(t_s + c, x);
+          tmem_wait_ld();
+          if (!full) hide(c, x);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) top = fmaxf(top, fmaf(x[e] * by, scales.k[c + e], scales.log_v[c + e]));
+        }
         if (__any_sync(0xffffffffu, top > m + kLazy)) raise(top);
         if (!ok) break;
         const float from = m == -INFINITY ? 0.f : m;
@@ -733,7 +839,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
           float x[32];
           tmem_ld_32(t_s + c, x);
           tmem_wait_ld();
-          if (!full) hide(c, x, 32);
+          if (!full) hide(c, x);
           uint32_t p[16];
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
@@ -783,14 +889,15 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
       }
       const bool theirs = keep1 > 0.f;  // stream 1 may not have had a tile: then its memory means nothing
       const float inverse = l == 0.f ? 0.f : 1.f / l;
-      T* dst = static_cast<T*>(a.out) + (u.r.start + (live ? i : u.i0) / a.group) * a.out_stride +
-               (u.head * a.group + (live ? i : u.i0) % a.group) * HD;
+      // The stream's queries, whose place the output takes on its way, have been used. (Stream 1's part ends in front of
+      // the values' ring, where a unit with one row tile goes.)
+      uint8_t* const out_tile = u.turns.two ? q_tile : smem + S::V;
       float* part = nullptr;
       if (a.splits > 1) {
         float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + split_unit_bytes(gridDim.x / a.splits));
         part = parts + size_t(blockIdx.x) * part_floats<HD>();
         if (live) *reinterpret_cast<float2*>(part + kUnit * HD + 2 * (i - u.i0)) = make_float2(m, l);
-        if (split == 0 && tid == 0)
+        if (split == 0 && row == 0 && stream == 0)
           static_cast<SplitUnit*>(a.workspace)[index] = {u.r.start, u.i0, u.rows, u.head};
       }
 #pragma unroll 1
@@ -805,6 +912,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
         }
         if (live && bars->odd) {
           // non-finite values of the masked tiles, added to the rows that see them
+          const RowMask mask = row_sees();
           const PageRows rows = {a.s.tables + u.seq * a.s.table_stride, a.c.page_shift, a.c.page_size - 1,
                                  a.c.num_pages, a.c.kv_heads, u.head, nullptr};
 #pragma unroll 1
@@ -828,14 +936,26 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
 #pragma unroll
           for (int e = 0; e < 32; e += 4)
             *reinterpret_cast<float4*>(part + size_t(i - u.i0) * HD + c + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
-        } else if (live) {
+        } else if (a.splits == 1) {
 #pragma unroll
           for (int e = 0; e < 32; e += 8)
-            *reinterpret_cast<uint4*>(dst + c + e) =
+            *reinterpret_cast<uint4*>(out_tile + tile_at(row, (c + e) / 8)) =
                 make_uint4(pack2<T>(x[e] * inverse, x[e + 1] * inverse), pack2<T>(x[e + 2] * inverse, x[e + 3] * inverse),
                            pack2<T>(x[e + 4] * inverse, x[e + 5] * inverse), pack2<T>(x[e + 6] * inverse, x[e + 7] * inverse));
         }
         __syncwarp();
+      }
+      if (a.splits == 1) {
+        if (stream == 0) named_barrier_sync(3, kRoleThreads);
+        else named_barrier_sync(4, kRoleThreads);
+        Walk at = walk;
+#pragma unroll 4
+        for (int p = 0; p < QV; ++p, at.advance(a.group)) {
+          if (at.packed < unit_rows)
+            *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (u.r.start + at.j) * a.out_stride +
+                                      (u.head * a.group + at.g) * HD + row % QV * 8) =
+                *reinterpret_cast<const uint4*>(out_tile + tile_at(row / QV + p * Walk::STEP, row % QV));
+        }
       }
     }
     tc_fence_before();
