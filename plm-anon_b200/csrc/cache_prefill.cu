@@ -8,12 +8,12 @@
 //     S[128, 128] = Q K^T     tcgen05.mma, both operands in shared memory, S in tensor memory;
 //     P = 2^(S scale - m)     a thread per row: S from tensor memory, P (16 bit) back over S's own columns;
 //     O[128, d] += P V        tcgen05.mma, P from tensor memory, V [key][d] as a transposed operand.
-// One thread issues P V and the next Q K' of whichever stream is ready, so one stream's two products (4 x 128 x 128 x d
-// flops) run under the other one's softmax. Products of one thread execute in order, so S may be overwritten as soon as the product
+// A thread for each stream issues its P V and the next Q K', so one stream's two products (4 x 128 x 128 x d flops) run
+// under the other one's softmax. Products of one thread execute in order, so S may be overwritten as soon as the product
 // that reads P has been issued.
 //
 // Roles: warps 0-3 and 4-7 do the softmax of stream 0 and 1, warps 8-11 fetch keys and values (16-bit pages by 16-byte
-// asynchronous copies, e4m3 codes through registers, exactly to f16), a thread of warp 12 issues the products. Operands lie
+// asynchronous copies, e4m3 codes through registers, exactly to f16), a thread of warp 12 and 13 issues the products of stream 0 and 1. Operands lie
 // in 128-byte rows with the 128-byte swizzle, d = 128 in two panels. Every wait is bounded.
 //
 // Softmax: base 2, lazy maximum (O is rescaled only when a score passes m by more than 2^15), scales of e4m3 pages kept
@@ -33,7 +33,7 @@ namespace {
 constexpr int kTile = 128;  // rows of a stream, and keys
 constexpr int kUnit = 2 * kTile;
 constexpr int kRoleThreads = 128;
-constexpr int kPrefillThreads = 3 * kRoleThreads + 32;
+constexpr int kPrefillThreads = 3 * kRoleThreads + 64;
 constexpr int kScaleSlots = 4;
 constexpr uint32_t kTmemColumns = 512;
 constexpr float kGuess = 4.f;  // log2 of how far the first weights may stay below 1
@@ -58,6 +58,7 @@ struct PrefillBarriers {
       scales_full[kScaleSlots];
   int one[kScaleSlots];  // whether the tile has one scale
   uint32_t tmem;
+  int issuing;  // held by the stream that issues products
   int odd;  // a value that is no number was met in a masked tile
 };
 static_assert(sizeof(PrefillBarriers) <= 256, "barriers");
@@ -142,10 +143,6 @@ struct Turns {
   int t_begin, t_end;  // the CTA's key tiles
   int sinks0, begin0, end0, sinks1, begin1, end1;
   // (Fields by stream, not arrays: an index known only at run time would put them into local memory.)
-  __device__ __forceinline__ bool active(int s, int t) const {
-    if (!two) return ((t - t_begin) & 1) == s;
-    return t < (s ? sinks1 : sinks0) || (t >= (s ? begin1 : begin0) && t < (s ? end1 : end0));
-  }
   // The stream's first tile from t on (t_end or more: none).
   __device__ __forceinline__ int next(int s, int t) const {
     if (!two) return t + (((t - t_begin) ^ s) & 1);
@@ -488,92 +485,84 @@ __device__ __forceinline__ void fetch_tiles(const CacheAttnArgs& a, const Unit& 
   }
 }
 
-// Whether a barrier's phase is complete, at once (mbar_try_wait may hold the thread for a while).
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-
-// Issues all products: one thread, so that nothing of its warp has to be brought together again after a wait. It looks
-// at the streams in turn and issues P V and the next Q K of the one whose softmax is over, together: two streams whose
-// products mixed would finish, and start their softmax, at the same time.
+// A stream's products: one thread each, with as little to do as can be (alone, a thread takes five or more clocks for an
+// instruction, and every one stands in the stream's chain Q K, softmax, P V).
 template <int HD, bool BF16>
-__device__ __forceinline__ void issue_products(const CacheAttnArgs& a, const Turns& turns, uint8_t* smem,
+__device__ __forceinline__ void issue_products(const CacheAttnArgs& a, const Turns& turns, const int stream, uint8_t* smem,
                                                PrefillBarriers* bars) {
   using S = PrefillSmem<HD>;
   constexpr uint32_t QK = umma_idesc_f16(kTile, kTile, BF16);
   constexpr uint32_t PV = umma_idesc_f16(kTile, HD, BF16) | (1u << 16);  // B transposed
   constexpr int PANEL = kTile * 128;
   constexpr int STEP = S::TILE >> 4;  // a tile, in a descriptor's units
-  const uint32_t tmem = bars->tmem;
-  const uint64_t q_desc = umma_desc_sw128(smem_u32(smem + S::Q)), k_desc = umma_desc_sw128(smem_u32(smem + S::K));
+  const bool two = turns.two != 0;
+  const uint32_t t_s = bars->tmem + stream * kTile, t_o = t_s + 2 * kTile;
+  const uint64_t q = umma_desc_sw128(smem_u32(smem + S::Q + (two ? stream : 0) * S::TILE));
+  const uint64_t k_desc = umma_desc_sw128(smem_u32(smem + S::K));
   const uint64_t v_desc = umma_desc_transposed(smem_u32(smem + S::V), PANEL);
-  const int t_begin = turns.t_begin, tiles = turns.t_end - t_begin;
-  auto scores = [&](int s, int n) {
-    const uint64_t q = q_desc + (turns.two ? s * STEP : 0), k = k_desc + (n & 1) * STEP;
-    const uint32_t d = tmem + s * kTile;
-#pragma unroll
-    for (int x = 0; x < HD / 16; ++x) {
-      const int at = ((x >> 2) * PANEL + (x & 3) * 32) >> 4;
-      umma_f16(d, q + at, k + at, QK, x > 0 ? 1u : 0u);
-    }
-    umma_commit(bars->s_full + s);
-    umma_commit(bars->k_empty + (n & 1));
-    if (!turns.active(1 - s, t_begin + n)) umma_commit(bars->k_empty + (n & 1));  // the other stream has no use for it
+  // Tile numbers within the CTA: this stream's sinks and range, and the other one's.
+  const int t0 = turns.t_begin, tiles = turns.t_end - t0;
+  const int sinks = (stream ? turns.sinks1 : turns.sinks0) - t0, begin = (stream ? turns.begin1 : turns.begin0) - t0,
+            end = min(tiles, (stream ? turns.end1 : turns.end0) - t0);
+  const int o_sinks = (stream ? turns.sinks0 : turns.sinks1) - t0, o_begin = (stream ? turns.begin0 : turns.begin1) - t0,
+            o_end = (stream ? turns.end0 : turns.end1) - t0;
+  auto next = [&](int n) {
+    if (!two) return n + ((n ^ stream) & 1);
+    if (n >= sinks) n = max(n, begin);
+    return n < end || n < sinks ? n : tiles;
+  };
+  auto release = [&](uint64_t* empty, int n) {  // both streams' arrivals, where the other one has no use for the tile
+    umma_commit(empty + (n & 1));
+    if (!two || !(n < o_sinks || (n >= o_begin && n < o_end))) umma_commit(empty + (n & 1));
   };
   if (!mbar_wait(&bars->q_ready, 0, a.err, kErrTimeoutPeer)) return;
-  // The stream looked at and the other one: its tile, that tile's number among the stream's, and whether its scores have
-  // been asked for (then the product with the values is next). Nothing is waited for here: a stream that is ahead may need
-  // a tile whose place the other one has yet to free.
-  struct State {
-    int n, count;
-    bool scored;
-  };
-  State now = {turns.next(0, t_begin) - t_begin, 0, false}, other = {turns.next(1, t_begin) - t_begin, 0, false};
-  int s = 0;
-  uint64_t since = 0;
-  uint32_t looks = 0;  // the timer takes longer to read than everything else here
-  while (now.n < tiles || other.n < tiles) {
-    ++looks;
-    if (now.n < tiles && now.scored && mbar_test(bars->p_ready + s, now.count & 1) &&
-        mbar_test(bars->v_full + (now.n & 1), (now.n >> 1) & 1)) {
-      tc_fence_after();
-      const uint64_t v = v_desc + (now.n & 1) * STEP;
-      const uint32_t p = tmem + s * kTile;
-#pragma unroll
-      for (int x = 0; x < kTile / 16; ++x)
-        umma_f16_ts(p + 2 * kTile, p + x * 8, v + ((x * 2048) >> 4), PV, now.count > 0 || x > 0 ? 1u : 0u);
-      umma_commit(bars->pv_done + s);
-      umma_commit(bars->v_empty + (now.n & 1));
-      if (!turns.active(1 - s, t_begin + now.n)) umma_commit(bars->v_empty + (now.n & 1));
-      now = {turns.next(s, t_begin + now.n + 1) - t_begin, now.count + 1, false};
-      looks = 0;
-    }
-    if (now.n < tiles && !now.scored && mbar_test(bars->k_full + (now.n & 1), (now.n >> 1) & 1)) {
-      tc_fence_after();
-      scores(s, now.n);
-      now.scored = true;
-      looks = 0;
-    }
-    if (looks >= 4096 && (looks & 4095) == 0) {
-      if (looks == 4096) since = global_timer_ns();
-      if (global_timer_ns() - since > kWaitLimitNs) {
+  int n = next(0);
+  // Products are issued one stream at a time, and P V together with the next Q K: were two streams' products to mix, both
+  // would end late, both softmaxes would run at the same time, and the tensor core would idle under them. The lock is never
+  // held over a wait.
+  auto lock = [&]() {
+    for (uint32_t looks = 1; atomicExch(&bars->issuing, 1) != 0; ++looks)
+      if (looks == (1u << 24)) {
         record_error(a.err, kErrTimeoutPeer);
-        return;
+        return false;
       }
+    return true;
+  };
+  auto unlock = [&]() { atomicExch(&bars->issuing, 0); };
+  bool locked = false;
+  for (int count = 0; n < tiles; ++count) {
+    const int at = n & 1;
+    if (!locked || !mbar_try_wait(bars->k_full + at, (n >> 1) & 1)) {
+      if (locked) unlock();
+      if (!mbar_wait(bars->k_full + at, (n >> 1) & 1, a.err, kErrTimeoutFull) || !lock()) return;
     }
-    const State x = now;
-    now = other;
-    other = x;
-    s ^= 1;
+    tc_fence_after();
+    const uint64_t k = k_desc + at * STEP;
+#pragma unroll
+    for (int x = 0; x < HD / 16; ++x) {
+      const int off = ((x >> 2) * PANEL + (x & 3) * 32) >> 4;
+      umma_f16(t_s, q + off, k + off, QK, x > 0 ? 1u : 0u);
+    }
+    unlock();
+    umma_commit(bars->s_full + stream);
+    release(bars->k_empty, n);
+    const int before = n;
+    n = next(n + 1);
+    if (!mbar_wait(bars->v_full + at, (before >> 1) & 1, a.err, kErrTimeoutFull) ||
+        !mbar_wait(bars->p_ready + stream, count & 1, a.err, kErrTimeoutPeer) || !lock())
+      return;
+    locked = true;
+    tc_fence_after();
+    const uint64_t v = v_desc + at * STEP;
+    const uint32_t first = count > 0 ? 1u : 0u;
+#pragma unroll
+    for (int x = 0; x < kTile / 16; ++x)
+      umma_f16_ts(t_o, t_s + x * 8, v + ((x * 2048) >> 4), PV, x > 0 ? 1u : first);
+    // at once: the next keys may wait for this tile's place
+    umma_commit(bars->pv_done + stream);
+    release(bars->v_empty, before);
   }
+  if (locked) unlock();
 }
 
 // A thread's packed rows when the threads of a stream go through its tile together, every N-th: as row of the sequence
@@ -613,6 +602,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
   }
   if (tid == 0) {
     mbar_init(&bars->q_ready, 8);
+    bars->issuing = 0;
     for (int i = 0; i < 2; ++i) {
       mbar_init(bars->k_full + i, 4);
       mbar_init(bars->k_empty + i, 2);
@@ -644,7 +634,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
   } else if (role == 3) {
     if (lane == 0) {
       const Turns turns = u.turns;
-      issue_products<HD, std::is_same<M, __nv_bfloat16>::value>(a, turns, smem, bars);
+      issue_products<HD, std::is_same<M, __nv_bfloat16>::value>(a, turns, warp & 1, smem, bars);
     }
   } else {
     const int stream = role;
@@ -770,7 +760,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
           tmem_st_16cols(t_o + c, z);
         }
       };
-      if (one) {
+      if constexpr (!E4M3) {
         // One pass with the maximum as it is, 0 for a row that has seen no key yet; should it prove too small, or the
         // guess too large, it is put right and the pass repeated.
         uint32_t p[kTile / 2];
@@ -821,34 +811,77 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_st_16cols(t_s + c * 16, p + c * 16);  // over scores that have been read
       } else {
-        float top = -INFINITY;
+        // Short loops, the tile's maximum first: beside the fetching warps' code the pass above, straight-line for all of
+        // the tile, is fetched anew by every warp (2048 rows over 8048 keys: 274 us instead of 244; for 16-bit pages the
+        // pass above is the faster one, 8191 windowed rows in 144 us instead of 156). The next 32 scores are on their
+        // way while 32 are in work.
+        float x0[32], x1[32];
+        auto each = [&](auto&& work) {
+          tmem_ld_32(t_s, x0);
 #pragma unroll 1
-        for (int c = 0; c < kTile; c += 32) {
-          float x[32];
-          tmem_ld_32(t_s + c, x);
-          tmem_wait_ld();
-          if (!full) hide(c, x);
+          for (int c = 0; c < kTile; c += 64) {
+            tmem_wait_ld();
+            tmem_ld_32(t_s + c + 32, x1);
+            if (!full) hide(c, x0);
+            work(c, x0);
+            tmem_wait_ld();
+            if (c + 64 < kTile) tmem_ld_32(t_s + c + 64, x0);
+            if (!full) hide(c + 32, x1);
+            work(c + 32, x1);
+          }
+        };
+        float top = -INFINITY;
+        if (one) {
+          each([&](int, const float(&x)[32]) {
+            float tops[4] = {top, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int e = 0; e < 32; ++e) top = fmaxf(top, fmaf(x[e] * by, scales.k[c + e], scales.log_v[c + e]));
+            for (int e = 0; e < 32; e += 8)
+#pragma unroll
+              for (int y = 0; y < 4; ++y) tops[y] = fmaxf(fmaxf(tops[y], x[e + 2 * y]), x[e + 2 * y + 1]);
+            top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+          });
+          if (top > -INFINITY) top = fmaf(top, by, add);
+        } else {
+          each([&](int c, const float(&x)[32]) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) top = fmaxf(top, fmaf(x[e] * by, scales.k[c + e], scales.log_v[c + e]));
+          });
         }
         if (__any_sync(0xffffffffu, top > m + kLazy)) raise(top);
         if (!ok) break;
         const float from = m == -INFINITY ? 0.f : m;
-#pragma unroll 1
-        for (int c = 0; c < kTile; c += 32) {
-          float x[32];
-          tmem_ld_32(t_s + c, x);
-          tmem_wait_ld();
-          if (!full) hide(c, x);
-          uint32_t p[16];
+        if (one) {
+          const f32x2 scale2 = pair(by, by), from2 = pair(add - from, add - from);
+          f32x2 sums[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+          each([&](int c, const float(&x)[32]) {
+            uint32_t p[16];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            x[e] = ex2(fmaf(x[e] * by, scales.k[c + e], scales.log_v[c + e]) - from);
-            l = fmaf(x[e], scales.inv_v[c + e], l);
-          }
+            for (int e = 0; e < 32; e += 2) {
+              float lo, hi;
+              unpair(fma2(pair(x[e], x[e + 1]), scale2, from2), lo, hi);
+              lo = ex2(lo);
+              hi = ex2(hi);
+              sums[(e >> 1) & 1] = add2(pair(lo, hi), sums[(e >> 1) & 1]);
+              p[e / 2] = pack2<M>(lo, hi);
+            }
+            tmem_st_16cols(t_s + c / 2, p);  // over scores that have been read
+          });
+          float lo, hi;
+          unpair(add2(sums[0], sums[1]), lo, hi);
+          l = fmaf(lo + hi, inv_v, l);
+        } else {
+          each([&](int c, const float(&x)[32]) {
+            uint32_t p[16];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) p[e] = pack2<M>(x[2 * e], x[2 * e + 1]);
-          tmem_st_16cols(t_s + c / 2, p);
+            for (int e = 0; e < 32; e += 2) {
+              const float lo = ex2(fmaf(x[e] * by, scales.k[c + e], scales.log_v[c + e]) - from);
+              const float hi = ex2(fmaf(x[e + 1] * by, scales.k[c + e + 1], scales.log_v[c + e + 1]) - from);
+              l = fmaf(lo, scales.inv_v[c + e], l);
+              l = fmaf(hi, scales.inv_v[c + e + 1], l);
+              p[e / 2] = pack2<M>(lo, hi);
+            }
+            tmem_st_16cols(t_s + c / 2, p);
+          });
         }
       }
       tmem_wait_st();
