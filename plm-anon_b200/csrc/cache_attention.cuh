@@ -165,14 +165,47 @@ __device__ __forceinline__ void widen(TileKeys& t, const RowMask& m) {
   t.full_end = min(t.full_end, m.last + 1);
 }
 
-// Four neighbouring elements of packed row i (row i / group, query head i % group of the kv head) of a sequence that
-// starts at row0, divided by the row's sum.
-template <typename T>
-__device__ __forceinline__ void store_row4(const CacheAttnArgs& a, int row0, int i, int head, int hd, int d, float4 sum,
-                                           float total) {
+// N neighbouring elements of packed row i (row i / group, query head i % group of the kv head) of a sequence that starts
+// at row0, divided by the row's sum.
+template <typename T, int N>
+__device__ __forceinline__ void store_row(const CacheAttnArgs& a, int row0, int i, int head, int hd, int d,
+                                          const float (&sum)[N], float total) {
   const float inv = total == 0.f ? 0.f : 1.f / total;
   T* dst = static_cast<T*>(a.out) + (row0 + i / a.group) * a.out_stride + (head * a.group + i % a.group) * hd + d;
-  *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(sum.x * inv, sum.y * inv), pack2<T>(sum.z * inv, sum.w * inv));
+#pragma unroll
+  for (int e = 0; e < N; e += 2) reinterpret_cast<uint32_t*>(dst)[e / 2] = pack2<T>(sum[e] * inv, sum[e + 1] * inv);
+}
+
+// Adds up the parts of a row in order and stores it: one warp. part(i) is part i's floats, its O row `at` floats in and
+// its (m, l) at `ml`. The maxima first, all at once, so that the parts' rows are on their way together.
+template <int HD, typename T, typename Part>
+__device__ __forceinline__ void join_row(const CacheAttnArgs& a, int count, Part part, int at, int ml, int row0, int i,
+                                         int head) {
+  const int lane = threadIdx.x & 31;
+  constexpr int N = HD / 32;
+  float top = -INFINITY;
+  for (int x = lane; x < count; x += 32) top = fmaxf(top, part(x)[ml]);
+  top = warp_max(top);
+  const float from = top == -INFINITY ? 0.f : top;
+  float sum[N] = {}, total = 0.f;
+  for (int base = 0; base < count; base += 32) {
+    float2 mine = make_float2(-INFINITY, 0.f);
+    if (base + lane < count) mine = *reinterpret_cast<const float2*>(part(base + lane) + ml);
+    const float f = ex2(mine.x - from);
+    const int here = min(32, count - base);
+#pragma unroll 8
+    for (int x = 0; x < here; ++x) {
+      const float* src = part(base + x) + at + lane * N;
+      float v[N];
+      if constexpr (N == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
+      else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
+      const float w = __shfl_sync(0xffffffffu, f, x);
+      total = fmaf(w, __shfl_sync(0xffffffffu, mine.y, x), total);
+#pragma unroll
+      for (int e = 0; e < N; ++e) sum[e] = fmaf(w, v[e], sum[e]);
+    }
+  }
+  store_row<T>(a, row0, i, head, HD, lane * N, sum, total);
 }
 
 }  // namespace plm

@@ -555,7 +555,8 @@ __global__ void __launch_bounds__(kThreads, E4M3 && NR == 1 ? 2 : 1) decode_atte
         total += f * pl[w][row];
       }
       if (complete) {
-        store_row4<T>(a, r.start, row, head, HD, d, sum, total);
+        const float x[4] = {sum.x, sum.y, sum.z, sum.w};
+        store_row<T>(a, r.start, row, head, HD, d, x, total);
       } else {
         *reinterpret_cast<float4*>(part + row * HD + d) = sum;
         if (d == 0) *reinterpret_cast<float2*>(part + ROWS * HD + 2 * row) = make_float2(top, total);
@@ -575,36 +576,18 @@ __global__ void __launch_bounds__(kThreads, E4M3 && NR == 1 ? 2 : 1) decode_atte
   if (EVEN && !begun && tid == 0) split_tiles[worker].count = 0;
 }
 
-// Joins the tiles that several workers hold parts of, a CTA for each worker that began one, in the workers' order.
+// Joins the tiles that several workers hold parts of, a CTA for each worker that began one, a warp to a row.
 template <int HD, typename T, int ROWS>
-__global__ void __launch_bounds__(kThreads) join_kernel(const CacheAttnArgs a) {
+__global__ void __launch_bounds__(32 * ROWS) join_kernel(const CacheAttnArgs a) {
   grid_dependency_wait();
   allow_dependents();
-  const int worker = blockIdx.x, workers = gridDim.x;
+  const int worker = blockIdx.x, workers = gridDim.x, row = threadIdx.x >> 5;
   const SplitTile t = static_cast<const SplitTile*>(a.workspace)[worker];
+  if (t.count == 0 || row >= t.rows) return;
   const float* partials = reinterpret_cast<const float*>(static_cast<const uint8_t*>(a.workspace) + split_tile_bytes(workers));
-  constexpr int Q4 = HD / 4;
-  if (t.count == 0) return;
-  for (int item = threadIdx.x; item < t.rows * Q4; item += kThreads) {
-    const int row = item / Q4, d = (item % Q4) * 4;
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    float top = -INFINITY, total = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < t.count; ++i) {
-      const float* part = partials + size_t(2 * (worker + i) + (i == 0 ? 1 : 0)) * partial_floats<ROWS, HD>();
-      const float2 ml = *reinterpret_cast<const float2*>(part + ROWS * HD + 2 * row);
-      const float4 x = *reinterpret_cast<const float4*>(part + row * HD + d);
-      const float now = fmaxf(top, ml.x), from = now == -INFINITY ? 0.f : now;
-      const float keep = ex2(top - from), f = ex2(ml.x - from);
-      top = now;
-      sum.x = sum.x * keep + f * x.x;
-      sum.y = sum.y * keep + f * x.y;
-      sum.z = sum.z * keep + f * x.z;
-      sum.w = sum.w * keep + f * x.w;
-      total = total * keep + f * ml.y;
-    }
-    store_row4<T>(a, t.row0, row, t.head, HD, d, sum, total);
-  }
+  join_row<HD, T>(
+      a, t.count, [&](int i) { return partials + size_t(2 * (worker + i) + (i == 0 ? 1 : 0)) * partial_floats<ROWS, HD>(); },
+      row * HD, ROWS * HD + 2 * row, t.row0, row, t.head);
 }
 
 bool one_row_tile(const CacheAttnArgs& a) { return int64_t(a.s.max_rows) * a.group <= 8; }
@@ -628,7 +611,7 @@ int launch_decode(const CacheAttnArgs& a, int workers, cudaStream_t stream) {
   const unsigned ctas = even ? unsigned(workers) : unsigned(a.s.n_seqs) * unsigned(a.c.kv_heads);
   const int done = check_cuda(launch(kernel, dim3(ctas), dim3(kThreads), SMEM, stream, true, a), "decode_attention_kernel");
   if (done != PLM_OK || !even || workers == 1) return done;
-  return check_cuda(launch(join_kernel<HD, T, 8 * NR>, dim3(ctas), dim3(kThreads), 0, stream, true, a), "join_kernel");
+  return check_cuda(launch(join_kernel<HD, T, 8 * NR>, dim3(ctas), dim3(32 * 8 * NR), 0, stream, true, a), "join_kernel");
 }
 
 template <int HD, typename T>

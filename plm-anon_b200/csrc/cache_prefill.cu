@@ -1000,37 +1000,19 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
   }
 }
 
-// Adds up the parts of a unit in order: blockIdx.x the unit, blockIdx.y 32 of its rows.
+// Adds up the parts of a unit: blockIdx.x the unit, blockIdx.y 8 of its rows, a warp to a row.
 template <int HD, typename T>
 __global__ void __launch_bounds__(256) join_parts_kernel(const CacheAttnArgs a) {
   grid_dependency_wait();
   allow_dependents();
   const SplitUnit u = static_cast<const SplitUnit*>(a.workspace)[blockIdx.x];
+  const int row = blockIdx.y * 8 + (threadIdx.x >> 5);
+  if (row >= u.rows) return;
   const float* parts =
       reinterpret_cast<const float*>(static_cast<const uint8_t*>(a.workspace) + split_unit_bytes(gridDim.x)) +
       size_t(blockIdx.x) * a.splits * part_floats<HD>();
-  constexpr int Q4 = HD / 4;
-  const int row_end = min(u.rows, int(blockIdx.y + 1) * 32);
-  for (int item = blockIdx.y * 32 * Q4 + threadIdx.x; item < row_end * Q4; item += 256) {
-    const int row = item / Q4, d = (item % Q4) * 4;
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    float top = -INFINITY, total = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < a.splits; ++i) {
-      const float* part = parts + size_t(i) * part_floats<HD>();
-      const float2 ml = *reinterpret_cast<const float2*>(part + kUnit * HD + 2 * row);
-      const float4 x = *reinterpret_cast<const float4*>(part + size_t(row) * HD + d);
-      const float now = fmaxf(top, ml.x), from = now == -INFINITY ? 0.f : now;
-      const float keep = ex2(top - from), f = ex2(ml.x - from);
-      top = now;
-      sum.x = sum.x * keep + f * x.x;
-      sum.y = sum.y * keep + f * x.y;
-      sum.z = sum.z * keep + f * x.z;
-      sum.w = sum.w * keep + f * x.w;
-      total = total * keep + f * ml.y;
-    }
-    store_row4<T>(a, u.row0, u.i0 + row, u.head, HD, d, sum, total);
-  }
+  join_row<HD, T>(a, a.splits, [&](int i) { return parts + size_t(i) * part_floats<HD>(); }, row * HD, kUnit * HD + 2 * row,
+                  u.row0, u.i0 + row, u.head);
 }
 
 // Units of a call, at most: a sequence has one more than its full ones.
@@ -1059,7 +1041,8 @@ int launch_prefill(CacheAttnArgs a, int64_t max_keys, int num_sms, cudaStream_t 
   st = check_cuda(launch(kernel, dim3(unsigned(units * a.splits)), dim3(kPrefillThreads), SMEM, stream, true, a),
                   "prefill_attention_kernel");
   if (st != PLM_OK || a.splits == 1) return st;
-  return check_cuda(launch(join_parts_kernel<HD, T>, dim3(unsigned(units), kUnit / 32), dim3(256), 0, stream, true, a),
+  const int rows = int(std::min<int64_t>(kUnit, (int64_t(a.s.max_rows) * a.group + 7) / 8 * 8));
+  return check_cuda(launch(join_parts_kernel<HD, T>, dim3(unsigned(units), rows / 8), dim3(256), 0, stream, true, a),
                     "join_parts_kernel");
 }
 
