@@ -18,6 +18,7 @@ What contradicts the host's bounds on the device (a row range, a page, a positio
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
@@ -25,6 +26,26 @@ from . import native
 from .native import NativeError
 
 MAX_SCALE_BLOCK = 64
+
+# A call's descriptor is packed from its own fields here and the finished bytes of its cache and sequences: a third of the
+# time of filling ctypes structures, and the smallest calls last as long as their host side.
+_APPEND = struct.Struct("@iiPPPqqqPqiiPP")    # plm_cache_append_desc up to the cache
+_ATTENTION = struct.Struct("@iiPqPqifiiPPPq")  # plm_cache_attention_desc up to the cache
+_entry_points: dict = {}
+
+
+def _entry(name: str, argtypes: list):
+    """A function of the library that takes its descriptor as bytes."""
+    fn = _entry_points.get(name)
+    if fn is None:
+        fn = native.library()[name]  # an object of its own, with a signature of its own
+        fn.argtypes, fn.restype = argtypes, ctypes.c_int32
+        _entry_points[name] = fn
+    return fn
+
+
+def _raw_stream(index: int, stream) -> int:
+    return torch._C._cuda_getCurrentRawStream(index) if stream is None else stream.cuda_stream
 _MODEL_DTYPES = {torch.bfloat16: native.PLM_BF16, torch.float16: native.PLM_F16}
 
 
@@ -67,6 +88,9 @@ class PagedCache:
             kind=native.CACHE_E4M3 if e4m3 else native.CACHE_MODEL, k=k.data_ptr(), v=v.data_ptr(),
             k_scale=native.ptr(k_scale), v_scale=native.ptr(v_scale), scale_block=block, num_pages=pages,
             page_size=page, num_kv_heads=kv_heads, head_dim=head_dim)
+        self._bytes = bytes(self.desc)
+        self._index = k.get_device()
+        self._workspaces: dict = {}  # bytes that an attention call of some sizes needs
 
     @classmethod
     def allocate(cls, num_pages: int, num_kv_heads: int, page_size: int, head_dim: int, *,
@@ -111,6 +135,8 @@ class Sequences:
             n_seqs=n, max_rows=max_rows, max_keys=max_keys, row_start=row_start.data_ptr(), context=context.data_ptr(),
             block_tables=block_tables.data_ptr(), table_stride=block_tables.stride(0) if n > 1 else pages,
             max_pages=pages)
+        self._bytes = bytes(self.desc)
+        self._index = row_start.get_device()
 
 
 def _heads(what: str, name: str, t: torch.Tensor, rows: int, heads: int | None, head_dim: int, dtype) -> int:
@@ -137,15 +163,15 @@ def _common(what: str, ctx, cache: PagedCache, seqs: Sequences, rows: int, dtype
     return code
 
 
-def _device(what: str, ctx, cache: PagedCache, seqs: Sequences, **tensors) -> torch.device:
+def _devices(what: str, ctx, cache: PagedCache, seqs: Sequences, **tensors) -> None:
+    """Raises for what is not on the context's device."""
     device = torch.device("cuda", ctx.device)
     _same_device(what, device, cache=cache, sequences=seqs, **tensors)
-    return device
 
 
-def _table(what: str, name: str, t: torch.Tensor | None, rows: int) -> int | None:
+def _table(what: str, name: str, t: torch.Tensor | None, rows: int) -> int:
     if t is None:
-        return None
+        return 0
     if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != rows or (rows > 1 and t.stride(0) != 1):
         raise NativeError(f"{what}: {name} is contiguous int32 [{rows}]")
     return t.data_ptr()
@@ -181,30 +207,34 @@ def append(ctx: native.Context, cache: PagedCache, seqs: Sequences, k: torch.Ten
     rows, hd = k.shape[0], cache.head_dim
     dtype = k.dtype
     code = _common(what, ctx, cache, seqs, rows, dtype)
-    desc = native.CacheAppendDesc(dtype=code, rows=rows, cache=cache.desc, seqs=seqs.desc)
-    desc.k_stride = _heads(what, "k", k, rows, cache.num_kv_heads, hd, dtype)
-    desc.v_stride = _heads(what, "v", v, rows, cache.num_kv_heads, hd, dtype)
+    k_stride = _heads(what, "k", k, rows, cache.num_kv_heads, hd, dtype)
+    v_stride = _heads(what, "v", v, rows, cache.num_kv_heads, hd, dtype)
+    heads = q_stride = q_out_stride = q_ptr = q_out_ptr = cos_ptr = max_pos = 0
     if q is not None:
-        desc.q_stride = _heads(what, "q", q, rows, None, hd, dtype)
-        desc.num_heads = q.shape[1]
-        if q_out is not None:
-            desc.q_out_stride = _heads(what, "q_out", q_out, rows, q.shape[1], hd, dtype)
+        q_stride = _heads(what, "q", q, rows, None, hd, dtype)
+        heads = q.shape[1]
+        q_out_stride = heads * hd if q_out is None else _heads(what, "q_out", q_out, rows, heads, hd, dtype)
     elif q_out is not None:
         raise NativeError(f"{what}: q_out without q")
     if cos_sin is not None:
         if cos_sin.dtype != dtype or cos_sin.dim() != 2 or cos_sin.shape[1] != hd or not cos_sin.is_contiguous():
             raise NativeError(f"{what}: cos_sin is contiguous {dtype} [max_pos, {hd}]")
-        desc.cos_sin, desc.max_pos = cos_sin.data_ptr(), cos_sin.shape[0]
-    desc.positions = _table(what, "positions", positions, rows)
-    device = _device(what, ctx, cache, seqs, k=k, v=v, q=q, q_out=q_out, cos_sin=cos_sin, positions=positions)
+        cos_ptr, max_pos = cos_sin.data_ptr(), cos_sin.shape[0]
+    positions_ptr = _table(what, "positions", positions, rows)
+    index = ctx.device
+    for t in (cache, seqs, k, v, q, q_out, cos_sin, positions):
+        if t is not None and (t._index if t is cache or t is seqs else t.get_device()) != index:
+            _devices(what, ctx, cache, seqs, k=k, v=v, q=q, q_out=q_out, cos_sin=cos_sin, positions=positions)
     if q is not None:
         if q_out is None:
             q_out = _output(q, stream)
-            desc.q_out_stride = q.shape[1] * hd
-        desc.q, desc.q_out = q.data_ptr(), q_out.data_ptr()
-    desc.k, desc.v = k.data_ptr(), v.data_ptr()
-    on = (stream if stream is not None else torch.cuda.current_stream(device)).cuda_stream
-    native.check(native.library().plm_cache_append(ctx.handle, ctypes.byref(desc), on), "plm_cache_append")
+        q_ptr, q_out_ptr = q.data_ptr(), q_out.data_ptr()
+    desc = _APPEND.pack(code, rows, q_ptr, k.data_ptr(), v.data_ptr(), q_stride, k_stride, v_stride, q_out_ptr,
+                        q_out_stride, heads, max_pos, cos_ptr, positions_ptr) + cache._bytes + seqs._bytes
+    status = _entry("plm_cache_append", [ctypes.c_void_p, ctypes.c_char_p, ctypes.c_void_p])(
+        ctx.handle, desc, _raw_stream(index, stream))
+    if status:
+        native.check(status, "plm_cache_append")
     return q_out
 
 
@@ -229,18 +259,36 @@ def attention(ctx: native.Context, cache: PagedCache, seqs: Sequences, q: torch.
         raise NativeError(f"{what}: scale {scale}")
     if (depth is None) != (own_start is None):
         raise NativeError(f"{what}: depth and own_start go together")
+    if not (0 <= window < 1 << 31 and 0 <= sinks < 1 << 31):
+        raise NativeError(f"{what}: window {window}, sinks {sinks}")
     depth_ptr, own_ptr = _table(what, "depth", depth, rows), _table(what, "own_start", own_start, rows)
-    device = _device(what, ctx, cache, seqs, q=q, out=out, depth=depth, own_start=own_start)
+    index = ctx.device
+    for t in (cache, seqs, q, out, depth, own_start):
+        if t is not None and (t._index if t is cache or t is seqs else t.get_device()) != index:
+            _devices(what, ctx, cache, seqs, q=q, out=out, depth=depth, own_start=own_start)
     if out is None:
         out = _output(q, stream)
-    desc = native.CacheAttentionDesc(
-        dtype=code, rows=rows, q=q.data_ptr(), q_stride=q_stride, out=out.data_ptr(), out_stride=out_stride,
-        num_heads=heads, scale=scale or 0.0, window=window, sinks=sinks, depth=depth_ptr, own_start=own_ptr,
-        cache=cache.desc, seqs=seqs.desc)
-    size = native.cache_attention_workspace(ctx, desc)
-    if size:
-        workspace = _scratch(size, device, stream)
-        desc.workspace, desc.workspace_bytes = workspace.data_ptr(), size
-    on = (stream if stream is not None else torch.cuda.current_stream(device)).cuda_stream
-    native.check(native.library().plm_cache_attention(ctx.handle, ctypes.byref(desc), on), "plm_cache_attention")
+    fields = (code, rows, q.data_ptr(), q_stride, out.data_ptr(), out_stride, heads, scale or 0.0, window, sinks, depth_ptr,
+              own_ptr)
+    tail = cache._bytes + seqs._bytes
+    sizes = (code, rows, heads, window, sinks, seqs.count, seqs.max_rows, seqs.max_keys, seqs.desc.max_pages)
+    size = cache._workspaces.get(sizes)
+    if size is None:
+        size = _workspace_bytes(ctx, _ATTENTION.pack(*fields, 0, 0) + tail)
+        if len(cache._workspaces) >= 256:  # sizes of calls long past
+            cache._workspaces.clear()
+        cache._workspaces[sizes] = size
+    workspace = _scratch(size, q.device, stream) if size else None
+    desc = _ATTENTION.pack(*fields, workspace.data_ptr() if size else 0, size) + tail
+    status = _entry("plm_cache_attention", [ctypes.c_void_p, ctypes.c_char_p, ctypes.c_void_p])(
+        ctx.handle, desc, _raw_stream(index, stream))
+    if status:
+        native.check(status, "plm_cache_attention")
     return out
+
+
+def _workspace_bytes(ctx, desc: bytes) -> int:
+    size = ctypes.c_int64(0)
+    native.check(_entry("plm_cache_attention_workspace", [ctypes.c_void_p, ctypes.c_char_p, ctypes.c_void_p])(
+        ctx.handle, desc, ctypes.addressof(size)), "plm_cache_attention_workspace")
+    return size.value

@@ -34,6 +34,18 @@ def test_structs_match_c_layout(tmp_path):
             assert int(sizes[f"{struct}.{field}"]) == getattr(mirror, field).offset, f"{struct}.{field}"
 
 
+def test_packed_descriptors_match_ctypes():
+    """plm.cache packs a call's own fields in front of the bytes of its cache and sequences."""
+    for pack, desc in ((api._APPEND, native.CacheAppendDesc), (api._ATTENTION, native.CacheAttentionDesc)):
+        own = [f for f, _ in desc._fields_ if f not in ("cache", "seqs")]
+        assert pack.size == desc.cache.offset
+        assert desc.seqs.offset == desc.cache.offset + ctypes.sizeof(native.PagedCacheDesc)
+        assert ctypes.sizeof(desc) == desc.seqs.offset + ctypes.sizeof(native.SequencesDesc)
+        values = list(range(1, len(own) + 1))
+        filled = desc.from_buffer_copy(pack.pack(*values) + bytes(ctypes.sizeof(desc) - pack.size))
+        assert [getattr(filled, f) for f in own] == values
+
+
 def _cache(dtype=torch.bfloat16, **kw):
     return api.PagedCache.allocate(4, 2, kw.pop("page", 16), kw.pop("head_dim", 64), dtype=dtype, device="cpu", **kw)
 
@@ -110,7 +122,7 @@ def test_attention_refusals():
     for kwargs in (dict(q=z(3, 3, 64)), dict(q=z(3, 4, 128)), dict(q=z(3, 4, 64, dtype=torch.float16)),
                    dict(q=z(3, 256)), dict(q=z(0, 4, 64)), dict(q=q, out=z(3, 2, 64)), dict(q=q, out=z(2, 4, 64)),
                    dict(q=q, scale=0.0), dict(q=q, scale=float("nan")), dict(q=q, scale=float("inf")),
-                   dict(q=q, depth=t), dict(q=q, own_start=t), dict(q=q, depth=t.long(), own_start=t),
+                   dict(q=q, window=-1), dict(q=q, sinks=1 << 31), dict(q=q, depth=t), dict(q=q, own_start=t), dict(q=q, depth=t.long(), own_start=t),
                    dict(q=q, depth=t[:2], own_start=t[:2])):
         with pytest.raises(NativeError):
             api.attention(ctx, cache, seqs, **kwargs)
