@@ -31,6 +31,17 @@ struct AppendArgs {
   int* err;
 };
 
+// Code `at` of a word of four.
+__device__ __forceinline__ float code_f32(uint32_t word, int at) {
+  const uint32_t h = e4m3x2_to_f16x2(uint16_t((word >> (8 * at)) & 0xffu));
+  return __low2float(*reinterpret_cast<const __half2*>(&h));
+}
+// Four values times `factor` as codes.
+__device__ __forceinline__ uint32_t pack_codes(const float* x, float factor) {
+  return uint32_t(f32x2_to_e4m3x2(x[0] * factor, x[1] * factor)) |
+         uint32_t(f32x2_to_e4m3x2(x[2] * factor, x[3] * factor)) << 16;
+}
+
 // 8 elements of the model dtype as floats.
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
@@ -162,57 +173,54 @@ __device__ __forceinline__ int locate_block(const CacheSeqs& s, int unit, int bl
   return -1;
 }
 
-// e4m3 pages: a CTA per (block of tokens, kv head, K or V) that the call's rows fall into holds the block's new values
-// in registers, agrees on their maximum, and writes scale and codes; the rest of the grid rotates queries.
-template <int HD, typename T>
-__global__ void __launch_bounds__(kAppendThreads) append_e4m3_kernel(const AppendArgs a) {
+// e4m3 pages: a CTA per (block of tokens, kv head) that the call's rows fall into, half of it for K and half for V. Each
+// half holds the block's new values in registers (PASSES times as many tokens as it covers at once), agrees on their
+// maximum, and writes scale and codes; the rest of the grid rotates queries. Bound by HBM for long prompts; what has to
+// follow what (sequence, rows and page, old scale, codes) is kept to one load each.
+template <int HD, typename T, int PASSES>
+__global__ void __launch_bounds__(2 * kAppendThreads) append_e4m3_kernel(const AppendArgs a) {
   constexpr int CH = HD / 16;
   constexpr int TOK = kAppendThreads / CH;  // tokens a pass over the block covers
-  constexpr int PASSES = kMaxScaleBlock / TOK;
-  __shared__ float warp_amax[kAppendThreads / 32];
+  __shared__ float warp_amax[2 * kAppendThreads / 32];
   grid_dependency_wait();
   allow_dependents();
-  const int tid = threadIdx.x, chunk = tid % CH;
   if (int(blockIdx.x) >= a.kv_units) {
-    const int64_t item = int64_t(int(blockIdx.x) - a.kv_units) * kAppendThreads + tid;
+    const int64_t item = int64_t(int(blockIdx.x) - a.kv_units) * 2 * kAppendThreads + threadIdx.x;
     const int64_t head_row = item / CH;
     if (head_row < int64_t(a.s.rows) * a.heads)
-      append_16bit<HD, T>(a, int(head_row / a.heads), int(head_row % a.heads), chunk);
+      append_16bit<HD, T>(a, int(head_row / a.heads), int(head_row % a.heads), int(item % CH));
     return;
   }
-  const int per_block = 2 * a.c.kv_heads;
-  const int slot = int(blockIdx.x) % per_block;
-  const bool key = slot < a.c.kv_heads;
-  const int head = key ? slot : slot - a.c.kv_heads;
+  const bool key = threadIdx.x < kAppendThreads;
+  const int tid = threadIdx.x % kAppendThreads, chunk = tid % CH;
+  const int head = int(blockIdx.x) % a.c.kv_heads;
   SeqRange r;
   int64_t block;
-  const int seq = locate_block(a.s, int(blockIdx.x) / per_block, a.c.block_shift, &r, &block, a.err);
+  const int seq = locate_block(a.s, int(blockIdx.x) / a.c.kv_heads, a.c.block_shift, &r, &block, a.err);
   if (seq < 0) return;
   const int size = 1 << a.c.block_shift;
   const int64_t first = block << a.c.block_shift;
-  const int page = physical_page(a.s, a.c, seq, first >> a.c.page_shift, a.err);
-  if (page < 0) return;
   const int begin = int(max(r.context - first, int64_t(0)));  // the block's tokens before this call
   const int end = int(min(r.context + r.n - first, int64_t(size)));
-  const size_t head_page = size_t(page) * a.c.kv_heads + head;
-  const int slot0 = int(first & (a.c.page_size - 1));
-  uint8_t* codes = static_cast<uint8_t*>(key ? a.c.k : a.c.v) + (head_page * a.c.page_size + slot0) * HD;
-  float* scale = (key ? a.c.k_scale : a.c.v_scale) + head_page * (a.c.page_size >> a.c.block_shift) +
-                 (slot0 >> a.c.block_shift);
-  const T* src = static_cast<const T*>(key ? a.k : a.v);
+  const T* src = static_cast<const T*>(key ? a.k : a.v) + head * HD + chunk * 8;
   const int64_t stride = key ? a.k_stride : a.v_stride;
 
   float lo[PASSES][8], hi[PASSES][8];
+#pragma unroll
+  for (int p = 0; p < PASSES; ++p) {
+    const int token = tid / CH + p * TOK;
+    if (token < begin || token >= end) continue;
+    const int64_t row = r.start + first + token - r.context;
+    load8<T>(src + row * stride, lo[p]);
+    load8<T>(src + row * stride + HD / 2, hi[p]);
+  }
+  const int page = physical_page(a.s, a.c, seq, first >> a.c.page_shift, a.err);
   float amax = 0.f;
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
     const int token = tid / CH + p * TOK;
     if (token < begin || token >= end) continue;
-    const int64_t logical = first + token;
-    const int row = r.start + int(logical - r.context);
-    load8<T>(src + row * stride + head * HD + chunk * 8, lo[p]);
-    load8<T>(src + row * stride + head * HD + HD / 2 + chunk * 8, hi[p]);
-    if (key) rotate<HD, T>(a, row, logical, chunk, lo[p], hi[p]);
+    if (key) rotate<HD, T>(a, int(r.start + first + token - r.context), first + token, chunk, lo[p], hi[p]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float x = fabsf(lo[p][e]), y = fabsf(hi[p][e]);
@@ -220,46 +228,46 @@ __global__ void __launch_bounds__(kAppendThreads) append_e4m3_kernel(const Appen
       if (y < INFINITY) amax = fmaxf(amax, y);
     }
   }
+  if (page < 0) return;  // the whole CTA
+  const size_t head_page = size_t(page) * a.c.kv_heads + head;
+  const int slot0 = int(first & (a.c.page_size - 1));
+  uint8_t* codes = static_cast<uint8_t*>(key ? a.c.k : a.c.v) + (head_page * a.c.page_size + slot0) * HD + chunk * 8;
+  float* scale = (key ? a.c.k_scale : a.c.v_scale) + head_page * (a.c.page_size >> a.c.block_shift) +
+                 (slot0 >> a.c.block_shift);
+  const float old = begin > 0 ? *scale : 0.f;
   amax = warp_max(amax);
-  if ((tid & 31) == 0) warp_amax[tid >> 5] = amax;
-  __syncthreads();
+  if ((tid & 31) == 0) warp_amax[threadIdx.x >> 5] = amax;
+  __syncthreads();  // also: every thread has read the old scale
 #pragma unroll
-  for (int w = 0; w < kAppendThreads / 32; ++w) amax = fmaxf(amax, warp_amax[w]);
-  const float wanted = exp2_int(scale_exponent(amax));
-  const float old = begin > 0 ? *scale : wanted;
-  const float now = begin > 0 ? fmaxf(wanted, old) : wanted;
+  for (int w = 0; w < kAppendThreads / 32; ++w) amax = fmaxf(amax, warp_amax[(key ? 0 : kAppendThreads / 32) + w]);
+  const float now = fmaxf(exp2_int(scale_exponent(amax)), old);
   const float inverse = 1.f / now;
-  __syncthreads();  // every thread has read the old scale
   if (tid == 0) *scale = now;
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
     const int token = tid / CH + p * TOK;
     if (token >= end) continue;
-    uint2* at_lo = reinterpret_cast<uint2*>(codes + token * HD + chunk * 8);
-    uint2* at_hi = reinterpret_cast<uint2*>(codes + token * HD + HD / 2 + chunk * 8);
+    uint2* at_lo = reinterpret_cast<uint2*>(codes + token * HD);
+    uint2* at_hi = reinterpret_cast<uint2*>(codes + token * HD + HD / 2);
     float factor = inverse;
     if (token < begin) {
       if (now == old) continue;
       const uint2 was[2] = {*at_lo, *at_hi};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const __half2 x = *reinterpret_cast<const __half2*>(&(const uint32_t&)e4m3x2_to_f16x2(reinterpret_cast<const uint16_t*>(&was[0])[e]));
-        const __half2 y = *reinterpret_cast<const __half2*>(&(const uint32_t&)e4m3x2_to_f16x2(reinterpret_cast<const uint16_t*>(&was[1])[e]));
-        lo[p][2 * e] = __low2float(x);
-        lo[p][2 * e + 1] = __high2float(x);
-        hi[p][2 * e] = __low2float(y);
-        hi[p][2 * e + 1] = __high2float(y);
+      for (int e = 0; e < 8; ++e) {
+        lo[p][e] = code_f32(e < 4 ? was[0].x : was[0].y, e & 3);
+        hi[p][e] = code_f32(e < 4 ? was[1].x : was[1].y, e & 3);
       }
       factor = old * inverse;
     }
-    uint16_t out[2][4];
+    uint32_t out[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      out[0][e] = f32x2_to_e4m3x2(lo[p][2 * e] * factor, lo[p][2 * e + 1] * factor);
-      out[1][e] = f32x2_to_e4m3x2(hi[p][2 * e] * factor, hi[p][2 * e + 1] * factor);
+    for (int e = 0; e < 2; ++e) {
+      out[e] = pack_codes(lo[p] + 4 * e, factor);
+      out[2 + e] = pack_codes(hi[p] + 4 * e, factor);
     }
-    *at_lo = make_uint2(uint32_t(out[0][0]) | uint32_t(out[0][1]) << 16, uint32_t(out[0][2]) | uint32_t(out[0][3]) << 16);
-    *at_hi = make_uint2(uint32_t(out[1][0]) | uint32_t(out[1][1]) << 16, uint32_t(out[1][2]) | uint32_t(out[1][3]) << 16);
+    *at_lo = make_uint2(out[0], out[1]);
+    *at_hi = make_uint2(out[2], out[3]);
   }
 }
 
@@ -275,11 +283,15 @@ int append_launch(AppendArgs a, int kind, cudaStream_t stream) {
   }
   // A sequence's rows touch at most rows blocks, and at most two more than its full ones.
   const int64_t blocks = std::min<int64_t>(a.s.rows, (a.s.rows >> a.c.block_shift) + 2 * int64_t(a.s.n_seqs));
-  const int64_t units = blocks * 2 * a.c.kv_heads;
-  const int64_t q_blocks = (int64_t(a.s.rows) * q_heads * CH + kAppendThreads - 1) / kAppendThreads;
+  const int64_t units = blocks * a.c.kv_heads;
+  constexpr int THREADS = 2 * kAppendThreads;
+  const int64_t q_blocks = (int64_t(a.s.rows) * q_heads * CH + THREADS - 1) / THREADS;
   a.kv_units = int(units);
-  return check_cuda(launch(append_e4m3_kernel<HD, T>, dim3(unsigned(units + q_blocks)), dim3(kAppendThreads), 0, stream,
-                           true, a),
+  constexpr int TOK = kAppendThreads / CH;
+  const int size = 1 << a.c.block_shift;
+  auto kernel = size <= TOK ? append_e4m3_kernel<HD, T, 1>
+                            : size <= 2 * TOK ? append_e4m3_kernel<HD, T, 2> : append_e4m3_kernel<HD, T, kMaxScaleBlock / TOK>;
+  return check_cuda(launch(kernel, dim3(unsigned(units + q_blocks)), dim3(THREADS), 0, stream, true, a),
                     "append_e4m3_kernel");
 }
 
