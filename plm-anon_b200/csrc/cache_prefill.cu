@@ -529,40 +529,56 @@ __device__ __forceinline__ void issue_products(const CacheAttnArgs& a, const Tur
     return true;
   };
   auto unlock = [&]() { atomicExch(&bars->issuing, 0); };
-  bool locked = false;
-  for (int count = 0; n < tiles; ++count) {
-    const int at = n & 1;
-    if (!locked || !mbar_try_wait(bars->k_full + at, (n >> 1) & 1)) {
-      if (locked) unlock();
-      if (!mbar_wait(bars->k_full + at, (n >> 1) & 1, a.err, kErrTimeoutFull) || !lock()) return;
-    }
-    tc_fence_after();
-    const uint64_t k = k_desc + at * STEP;
+  auto scores = [&](int n) {
+    const uint64_t k = k_desc + (n & 1) * STEP;
 #pragma unroll
     for (int x = 0; x < HD / 16; ++x) {
       const int off = ((x >> 2) * PANEL + (x & 3) * 32) >> 4;
       umma_f16(t_s, q + off, k + off, QK, x > 0 ? 1u : 0u);
     }
-    unlock();
-    umma_commit(bars->s_full + stream);
-    release(bars->k_empty, n);
-    const int before = n;
-    n = next(n + 1);
-    if (!mbar_wait(bars->v_full + at, (before >> 1) & 1, a.err, kErrTimeoutFull) ||
+  };
+  if (n >= tiles) return;
+  if (!mbar_wait(bars->k_full + (n & 1), (n >> 1) & 1, a.err, kErrTimeoutFull) || !lock()) return;
+  tc_fence_after();
+  scores(n);
+  unlock();
+  umma_commit(bars->s_full + stream);
+  release(bars->k_empty, n);
+  for (int count = 0;; ++count) {
+    const int after = next(n + 1), at = n & 1;
+    if (!mbar_wait(bars->v_full + at, (n >> 1) & 1, a.err, kErrTimeoutFull) ||
         !mbar_wait(bars->p_ready + stream, count & 1, a.err, kErrTimeoutPeer) || !lock())
       return;
-    locked = true;
     tc_fence_after();
     const uint64_t v = v_desc + at * STEP;
     const uint32_t first = count > 0 ? 1u : 0u;
 #pragma unroll
     for (int x = 0; x < kTile / 16; ++x)
       umma_f16_ts(t_o, t_s + x * 8, v + ((x * 2048) >> 4), PV, x > 0 ? 1u : first);
-    // at once: the next keys may wait for this tile's place
-    umma_commit(bars->pv_done + stream);
-    release(bars->v_empty, before);
+    // Commits take their time; but without its keys the next product may be waiting for this tile's place.
+    const bool ready = after < tiles && mbar_try_wait(bars->k_full + (after & 1), (after >> 1) & 1);
+    if (ready) {
+      tc_fence_after();
+      scores(after);
+      unlock();
+      umma_commit(bars->s_full + stream);
+      umma_commit(bars->pv_done + stream);
+      release(bars->v_empty, n);
+      release(bars->k_empty, after);
+    } else {
+      unlock();
+      umma_commit(bars->pv_done + stream);
+      release(bars->v_empty, n);
+      if (after >= tiles) return;
+      if (!mbar_wait(bars->k_full + (after & 1), (after >> 1) & 1, a.err, kErrTimeoutFull) || !lock()) return;
+      tc_fence_after();
+      scores(after);
+      unlock();
+      umma_commit(bars->s_full + stream);
+      release(bars->k_empty, after);
+    }
+    n = after;
   }
-  if (locked) unlock();
 }
 
 // A thread's packed rows when the threads of a stream go through its tile together, every N-th: as row of the sequence
