@@ -593,12 +593,15 @@ __global__ void __launch_bounds__(32 * ROWS) join_kernel(const CacheAttnArgs a) 
 bool one_row_tile(const CacheAttnArgs& a) { return int64_t(a.s.max_rows) * a.group <= 8; }
 
 // Workers of an even launch: the CTAs that are resident at once, or fewer where each would get less than two chunks a
-// warp.
+// warp. Where that takes little away, as many to every tile: tiles of one length then begin with a worker, which has one
+// tile to fetch queries for and to join (8 windows of 4096 keys, 64 tiles on 148 SMs: 128 workers 29.5 us, 148 workers 32.0).
 int decode_workers(const CacheAttnArgs& a, int kind, int64_t max_keys, int num_sms) {
   const int64_t keys = a.window > 0 ? std::min<int64_t>(max_keys, int64_t(a.window) + a.sinks + a.s.max_rows) : max_keys;
-  const int64_t chunks = int64_t(a.s.n_seqs) * a.c.kv_heads * ((keys + kChunk - 1) / kChunk);
+  const int64_t tiles = int64_t(a.s.n_seqs) * a.c.kv_heads, chunks = tiles * ((keys + kChunk - 1) / kChunk);
   const int64_t resident = num_sms * (kind == PLM_CACHE_E4M3 && one_row_tile(a) ? 2 : 1);
-  return int(std::max<int64_t>(1, std::min<int64_t>(resident, chunks / (2 * kWarps))));
+  const int64_t workers = std::max<int64_t>(1, std::min<int64_t>(resident, chunks / (2 * kWarps)));
+  const int64_t whole = workers / tiles * tiles;
+  return int(whole * 100 >= workers * 85 ? whole : workers);
 }
 
 template <int HD, typename T, bool E4M3, int NR>
