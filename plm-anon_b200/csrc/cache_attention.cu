@@ -31,7 +31,7 @@ int attention_arguments(plm_ctx* ctx, const plm_cache_attention_desc* d, CacheAt
     return fail(PLM_ERR_INVALID, "plm_cache_attention: depth and own_start go together");
   if (!(d->scale >= 0.f && d->scale < INFINITY))
     return fail(PLM_ERR_INVALID, "plm_cache_attention: scale %g", double(d->scale));
-  if (int64_t(d->rows) * d->num_heads >= (int64_t(1) << 31))
+  if (int64_t(d->rows) * d->num_heads >= (int64_t(1) << 30))
     return fail(PLM_ERR_UNSUPPORTED, "plm_cache_attention: %d rows of %d heads in one call", d->rows, d->num_heads);
   a.q = d->q;
   a.q_stride = d->q_stride;

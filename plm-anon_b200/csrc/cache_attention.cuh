@@ -158,7 +158,7 @@ __device__ __forceinline__ TileKeys causal_keys(const CacheAttnArgs& a, const Se
   return t;
 }
 
-// Of rows masked by depth and own_start, row by row with a stride: `step` threads see the rows from `first` on.
+// One more row, masked by depth and own_start (starting from lo and full_end kUnreachable, full_lo 0).
 __device__ __forceinline__ void widen(TileKeys& t, const RowMask& m) {
   t.lo = min(t.lo, min(m.first, m.own_first));
   t.full_lo = max(t.full_lo, m.first);

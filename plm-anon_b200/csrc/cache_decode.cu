@@ -145,6 +145,7 @@ __device__ __forceinline__ TileKeys few_rows_keys(const CacheAttnArgs& a, const 
     t.lo = t.full_end = kUnreachable;
     t.full_lo = 0;
     for (int j = 0; j < r.n; ++j) widen(t, row_mask(a, r, j));
+    t.lo = min(t.lo, t.end);
     t.sinks = min(a.sinks, t.lo);
   }
   t.count<kChunk>();

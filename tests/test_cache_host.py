@@ -182,3 +182,17 @@ def test_c_entry_points_refuse_null():
     assert lib.plm_cache_attention(None, ctypes.byref(attend), None) == -1
     assert lib.plm_cache_append(ctypes.addressof(_BLOCK), None, None) == -1
     assert lib.plm_cache_attention(ctypes.addressof(_BLOCK), None, None) == -1
+    assert lib.plm_cache_attention_workspace(None, ctypes.byref(attend), ctypes.byref(ctypes.c_int64())) == -1
+    assert lib.plm_cache_attention_workspace(ctypes.addressof(_BLOCK), ctypes.byref(attend), None) == -1
+
+
+def test_c_attention_refuses_a_missing_workspace():
+    """A call that has to share out its keys needs scratch of its own; a block of zeros has no SMs, and so one worker."""
+    _, attend = _descs()
+    lib, needed = native.library(), ctypes.c_int64(0)
+    assert lib.plm_cache_attention_workspace(ctypes.addressof(_BLOCK), ctypes.byref(attend), ctypes.byref(needed)) == 0
+    assert needed.value > 0
+    for workspace, size in ((None, 1 << 30), (A, needed.value - 1), (A + 4, 1 << 30)):
+        attend.workspace, attend.workspace_bytes = workspace, size
+        assert lib.plm_cache_attention(ctypes.addressof(_BLOCK), ctypes.byref(attend), None) == -1
+        assert "workspace" in native.last_error()

@@ -136,6 +136,10 @@ PAGES = [pytest.param("bf16", False, id="bf16"), pytest.param("f16", False, id="
     ([129], [511], 6, 2, 64, 16),
     ([300], [77], 4, 1, 128, 16),
     ([513, 1, 40], [0, 600, 129], 4, 2, 64, 32),
+    ([1, 2], [77, 30], 2, 1, 128, 1), ([40, 3], [20, 130], 2, 1, 64, 1), ([1], [300], 2, 2, 64, 8),
+    ([140], [9], 2, 2, 128, 4), ([30, 1], [5000, 4100], 2, 1, 128, 4096),
+    ([20] * 40, list(range(0, 400, 10)), 2, 2, 64, 16),        # more sequences than a warp has lanes
+    ([300] * 3, [1500, 0, 700], 16, 2, 128, 64),               # many units of a group of 8
 ])
 def test_attention_causal(ctx, dtype, e4m3, rows, context, heads, kv_heads, head_dim, page):
     st = Setup(rows=rows, context=context, kv_heads=kv_heads, head_dim=head_dim, page=page, dtype=dtype, e4m3=e4m3,
@@ -206,6 +210,31 @@ def test_attention_masked_tokens_may_hold_anything(ctx, dtype, e4m3, rows, conte
     assert torch.isnan(out[n - 1, 0]).all()
 
 
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_attention_many_sequences(ctx, e4m3):
+    """More sequences than one even launch takes: every tile a CTA of its own."""
+    from plm import cache as api
+
+    n = 1100
+    st = Setup(rows=[1, 0] * (n // 2), context=[(7 * i) % 90 for i in range(n)], kv_heads=1, head_dim=64, page=16,
+               dtype="bf16", e4m3=e4m3, seed=n)
+    q = st.randn(st.held, 2, 64)
+    out = api.attention(ctx, st.cache, st.seqs, q)
+    ctx.check()
+    want, bound = st.expected(q)
+    assert within(out, want, bound)
+
+
+@pytest.mark.parametrize("rows", [3, 40, 200])
+def test_attention_positions_far_ahead(ctx, rows):
+    """A depth far past the keys moves the window behind all of them: the sinks alone stay visible."""
+    st = Setup(rows=[rows], context=[50], kv_heads=2, head_dim=128, page=16, dtype="bf16", e4m3=False, seed=rows)
+    depth = torch.full((rows,), 1 << 30, dtype=torch.int32, device="cuda")
+    own = torch.full((rows,), 1 << 30, dtype=torch.int32, device="cuda")
+    _check_attention(ctx, st, 2, window=10, sinks=(1 << 31) - 1, depth=depth, own_start=own)
+    _check_attention(ctx, st, 2, window=10, sinks=3, depth=depth, own_start=own)
+
+
 @pytest.mark.parametrize("rows", [1, 60, 200])
 def test_attention_scales_far_apart(ctx, rows):
     """Scales of a sequence's blocks over 2^50: the weights' rounding stays relative to the largest term."""
@@ -217,6 +246,12 @@ def test_attention_scales_far_apart(ctx, rows):
     # and scales that are no powers of two
     st.cache.v_scale.uniform_(0.001, 1.0, generator=g)
     st.cache.k_scale.uniform_(0.001, 0.02, generator=g)
+    _check_attention(ctx, st, 2)
+    # keys' scales alone over 2^40, and both a little apart
+    st.cache.v_scale.fill_(2.0 ** -6)
+    st.cache.k_scale.copy_(torch.exp2(torch.randint(-48, -7, st.cache.k_scale.shape, generator=g, device="cuda").float()))
+    _check_attention(ctx, st, 2)
+    st.cache.v_scale.copy_(torch.exp2(torch.randint(-20, -8, st.cache.k_scale.shape, generator=g, device="cuda").float()))
     _check_attention(ctx, st, 2)
 
 
