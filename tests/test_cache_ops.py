@@ -24,6 +24,7 @@ class Setup:
                  spread=1.0):
         from plm import cache as api
 
+        block = min(block, page)
         g = torch.Generator(device="cuda").manual_seed(seed)
         self.rows, self.ctx_host, self.dtype = rows, context, DTYPES[dtype]
         need = [max(1, -(-(n + c) // page)) for n, c in zip(rows, context)]
