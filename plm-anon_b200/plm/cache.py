@@ -65,6 +65,8 @@ class PagedCache:
             raise NativeError("PagedCache: k and v are [num_pages, kv_heads, page_size, head_dim] of one shape and dtype")
         if not (k.is_contiguous() and v.is_contiguous()):
             raise NativeError("PagedCache: k and v must be contiguous")
+        if k.numel() == 0:
+            raise NativeError(f"PagedCache: pages of {list(k.shape)}")
         pages, kv_heads, page, head_dim = k.shape
         e4m3 = k.dtype == torch.float8_e4m3fn
         if not e4m3 and k.dtype not in _MODEL_DTYPES:
@@ -125,7 +127,7 @@ class Sequences:
         if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.shape[0] != n or \
                 block_tables.shape[1] < 1 or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1):
             raise NativeError("Sequences: block_tables is int32 [n, max_pages] with contiguous rows")
-        if max_rows < 1 or max_keys < 0:
+        if not (1 <= max_rows < 1 << 31 and 0 <= max_keys < 1 << 63):
             raise NativeError(f"Sequences: at most {max_rows} rows and {max_keys} keys to a sequence")
         _same_device("Sequences", row_start.device, context=context, block_tables=block_tables)
         self.row_start, self.context, self.block_tables = row_start, context, block_tables
@@ -144,6 +146,8 @@ def _heads(what: str, name: str, t: torch.Tensor, rows: int, heads: int | None, 
     shape = t.shape
     if len(shape) != 3 or shape[0] != rows or shape[2] != head_dim or (heads is not None and shape[1] != heads):
         raise NativeError(f"{what}: {name} is {list(shape)}, not [{rows}, {heads or 'heads'}, {head_dim}]")
+    if shape[1] < 1:
+        raise NativeError(f"{what}: {name} has no heads")
     if t.dtype != dtype:
         raise NativeError(f"{what}: {name} is {t.dtype}, not {dtype}")
     stride = t.stride()
@@ -217,7 +221,8 @@ def append(ctx: native.Context, cache: PagedCache, seqs: Sequences, k: torch.Ten
     elif q_out is not None:
         raise NativeError(f"{what}: q_out without q")
     if cos_sin is not None:
-        if cos_sin.dtype != dtype or cos_sin.dim() != 2 or cos_sin.shape[1] != hd or not cos_sin.is_contiguous():
+        if cos_sin.dtype != dtype or cos_sin.dim() != 2 or cos_sin.shape[1] != hd or not cos_sin.is_contiguous() or \
+                cos_sin.shape[0] < 1:
             raise NativeError(f"{what}: cos_sin is contiguous {dtype} [max_pos, {hd}]")
         cos_ptr, max_pos = cos_sin.data_ptr(), cos_sin.shape[0]
     positions_ptr = _table(what, "positions", positions, rows)
@@ -255,7 +260,7 @@ def attention(ctx: native.Context, cache: PagedCache, seqs: Sequences, q: torch.
     if heads % cache.num_kv_heads:
         raise NativeError(f"{what}: {heads} heads over {cache.num_kv_heads} kv heads")
     out_stride = _heads(what, "out", out, rows, heads, hd, dtype) if out is not None else heads * hd
-    if scale is not None and not 0.0 < scale < float("inf"):
+    if scale is not None and not 2.0 ** -126 <= scale < 2.0 ** 128:  # an fp32 number; 0 asks for the default
         raise NativeError(f"{what}: scale {scale}")
     if (depth is None) != (own_start is None):
         raise NativeError(f"{what}: depth and own_start go together")

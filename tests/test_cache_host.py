@@ -130,6 +130,26 @@ def test_attention_refusals():
         api.attention(ctx, cache, seqs, q)
 
 
+def test_what_would_pass_for_a_default_is_refused():
+    """Numbers that become 0 in their C type, and empty tensors, whose address is null: neither stands for "none"."""
+    ctx, cache, seqs = _NoContext(), _cache(), _seqs()
+    z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)  # noqa: E731
+    k = z(3, 2, 64)
+    for scale in (1e-50, 1e39):
+        with pytest.raises(NativeError, match="scale"):
+            api.attention(ctx, cache, seqs, z(3, 4, 64), scale=scale)
+    with pytest.raises(NativeError, match="cos_sin"):
+        api.append(ctx, cache, seqs, k, k, cos_sin=z(0, 64))
+    with pytest.raises(NativeError, match="no heads"):
+        api.append(ctx, cache, seqs, k, k, q=z(3, 0, 64))
+    with pytest.raises(NativeError, match="no heads"):
+        api.attention(ctx, cache, seqs, z(3, 0, 64))
+    with pytest.raises(NativeError, match="at most"):
+        _seqs(max_rows=(1 << 32) + 1)
+    with pytest.raises(NativeError, match="pages of"):
+        api.PagedCache(z(4, 0, 16, 64), z(4, 0, 16, 64))
+
+
 # ---- the C entry points: a zeroed block stands for the context, which no refusal reads
 _BLOCK = ctypes.create_string_buffer(512)
 A = 1 << 20  # some 16-byte aligned address
