@@ -1,8 +1,10 @@
 // Attention over a paged cache for sequences of few rows (at most 16 packed rows: rows times query heads per kv head).
 // Every key and value is read once, 2 d bytes of e4m3 codes or 4 d of 16-bit numbers.
 //
-// What bounds it: HBM in part, and the instructions that bring 16 keys through a warp, 427 with e4m3 pages (75 of them
-// turn codes into f16) and 350 with 16-bit pages. Measured, head_dim 128, both launches: one token at 32768 e4m3 keys, 16
+// What bounds it: with e4m3 pages the instructions that bring 16 keys through a warp, 427 (75 of them turn codes into
+// f16), two a clock on an SM whose schedulers are busy half of the time with 16 warps; with 16-bit pages (350) they are
+// busy a quarter of the time with 8 warps, 12 gain 1.5 %, and start, tail and join are what is left around the bytes.
+// Measured, head_dim 128, both launches: one token at 32768 e4m3 keys, 16
 // kv heads, 34.9 us (3.85 TB/s); one token of each of 61 sequences, 2 to 8191 e4m3 keys, 32 heads over 8, 121 us
 // (4.1 TB/s); of 8 sequences behind windows of 4096 16-bit keys, 32 heads over 8, 29.5 us (4.55 TB/s). One token at 1024
 // keys takes 9.8 us, all latency: few chunks to a warp, and join_kernel is a second launch.

@@ -18,8 +18,11 @@
 //
 // What bounds it: the chain of a stream, Q K (650 clocks from the first issue to the last product accepted, 250 more to
 // the waiting warps), softmax (2300: 128 exponentials a thread at 8 clocks a warp are 1024 of them), P V (620), commits
-// and barriers (700), 4.8 thousand for 128 keys; two streams side by side keep the tensor core at 45 % of the 2130 clocks
-// their four products take. The first tile is in softmax 7 thousand clocks after the CTA starts, the output takes 6.
+// and barriers (700), 4.8 thousand for 128 keys of 16-bit pages against the 2130 clocks that the four products of two
+// streams take. With e4m3 pages it is 7 thousand: softmax goes in two short loops, and the fetching warps bring codes to
+// f16 on the same schedulers. The first tile is in softmax 7 thousand clocks after the CTA starts, the output takes 6, so
+// the tensor core is busy 30 % of a call. With one row tile the rings of two hold one key tile for each stream, whose next
+// one is fetched late: 4 us a key tile and CTA (16 heads, 56 rows: 17 us over 256 keys, 32 over 4152, 77 over 16440).
 // Measured: 2048 rows, 16 heads, over 6000 + 2048 e4m3 keys 227 us (520 TFLOP/s, 32 % of a large bf16 product's rate);
 // 8191 rows, 16 heads over 4, window 1024, 139 us (465 TFLOP/s of visible pairs).
 //
