@@ -10,10 +10,11 @@
 // keys takes 9.8 us, all latency: few chunks to a warp, and join_kernel is a second launch.
 //
 // All chunks of 16 keys of all (sequence, kv head) tiles form one list, and the workers, the CTAs that fit on the GPU at
-// once, get equal shares of it, so uneven lengths and few heads keep every SM busy. A tile that a worker has to itself
-// goes to the output; the parts of one that several hold go to the workspace, and join_kernel, launched behind, adds them
-// up in the workers' order. (Clusters that share a tile through distributed shared memory leave SMs idle: 16 tiles x 8
-// CTAs, one to an SM, do not all find a place at once on 148 SMs in GPCs of at most 20.)
+// once, get equal shares of it, so uneven lengths and few heads keep every SM busy. The host sizes the grid by its bound on
+// the keys; where the sequences have fewer chunks than that makes workers, the first ones get a chunk each and the others
+// none. A tile that a worker has to itself goes to the output; the parts of one that several hold go to the workspace, and
+// join_kernel, launched behind, adds them up in the workers' order. (Clusters that share a tile through distributed shared
+// memory leave SMs idle: 16 tiles x 8 CTAs, one to an SM, do not all find a place at once on 148 SMs in GPCs of at most 20.)
 //
 // Within a worker the warps take turns at the chunks. Everything is transposed, keys and head elements on the M side of
 // mma.m16n8k16, packed rows on the N side:
@@ -182,6 +183,7 @@ __global__ void __launch_bounds__(kThreads, E4M3 && NR == 1 ? 2 : 1) decode_atte
 
   // ---- this worker's share [at, at_end) of all chunks, in the order of sequences, kv heads and keys
   int64_t all = 0, at = 0, at_end = 1;
+  int sharers = 1;  // workers that get a share: no more than there are chunks, as all that hold a part of a tile write one
   if constexpr (EVEN) {
     for (int i = tid; i < a.s.n_seqs; i += kThreads) {
       const SeqRange r = sequence_range(a.s, i, a.err);
@@ -204,8 +206,9 @@ __global__ void __launch_bounds__(kThreads, E4M3 && NR == 1 ? 2 : 1) decode_atte
     }
     __syncthreads();
     all = upto[a.s.n_seqs - 1] * a.c.kv_heads;
-    at = all * worker / workers;
-    at_end = all * (worker + 1) / workers;
+    sharers = int(min(int64_t(workers), all));
+    at = worker < sharers ? all * worker / sharers : 0;
+    at_end = worker < sharers ? all * (worker + 1) / sharers : 0;
   }
   SplitTile* const split_tiles = reinterpret_cast<SplitTile*>(a.workspace);
   float* const partials = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + split_tile_bytes(workers));
@@ -573,10 +576,10 @@ __global__ void __launch_bounds__(kThreads, E4M3 && NR == 1 ? 2 : 1) decode_atte
     }
     if (EVEN && !complete && c_begin == 0) {
       begun = true;
-      // its last chunk belongs to the largest worker w with all w / workers <= that chunk's index
+      // its last chunk belongs to the largest worker w with all w / sharers <= that chunk's index
       const int64_t last = at + t.chunks - 1;
       if (tid == 0)
-        split_tiles[worker] = {int(((last + 1) * workers - 1) / all) - worker + 1, r.start, rows, head};
+        split_tiles[worker] = {int(((last + 1) * sharers - 1) / all) - worker + 1, r.start, rows, head};
     }
     if (!EVEN) return;
     at += c_end - c_begin;

@@ -1,0 +1,114 @@
+"""The paged-cache operators where the host's bounds and the device's lengths are far apart, where a mask leaves a row or a
+sequence nothing, and at the ends of their number ranges; against the definitions in 64 bits (cache_reference.py)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests.cache_reference import within
+from tests.test_cache_ops import PAGES, Setup, _assert_pages, _bits
+
+pytestmark = pytest.mark.gpu
+
+
+def _int32(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def _loose(st, max_keys):
+    """The sequences of ``st`` with block tables for ``max_keys`` tokens and that bound (or, given by the tables, none)."""
+    from plm import cache as api
+
+    narrow = st.seqs.block_tables
+    wide = torch.full((narrow.shape[0], max_keys // st.cache.page_size), -1, dtype=torch.int32, device="cuda")
+    wide[:, :narrow.shape[1]] = narrow
+    return [api.Sequences(st.seqs.row_start, st.seqs.context, wide, max_rows=st.seqs.max_rows, max_keys=bound)
+            for bound in (max_keys, 0)]
+
+
+@pytest.fixture(params=[0xFF, 0x71], ids=["nan", "huge"])
+def hostile(request, monkeypatch):
+    """Every workspace of a call full of NaN, or of numbers near 1.2e30: what nobody has written shows."""
+    from plm import cache as api
+
+    plain = api._scratch
+
+    def scratch(size, device, stream):
+        return plain(size, device, stream).fill_(request.param)
+
+    monkeypatch.setattr(api, "_scratch", scratch)
+
+
+@pytest.mark.parametrize("dtype,e4m3", PAGES)
+@pytest.mark.parametrize("rows,context,heads,kv_heads,max_keys,options", [
+    ([1], [99], 16, 16, 8192, {}), ([1], [199], 32, 8, 32768, {}), ([1], [16], 1, 1, 8192, {}),
+    ([1], [299], 2, 1, 32768, {}), ([1] * 4, [49] * 4, 8, 8, 32768, {}), ([1] * 8, [17, 300, 45, 0, 80, 16, 15, 130], 2, 2, 8192, {}),
+    ([2] * 3, [250, 17, 60], 16, 2, 8192, {}),                             # 16 packed rows: the wider tile
+    ([0] * 31 + [1] + [0] * 32, [511] * 64, 8, 8, 512, {}),                # slots of which one holds a row
+    ([1] * 2, [120, 40], 8, 8, 32768, dict(window=4096, sinks=4)),         # contexts short of the window
+])
+def test_decode_of_keys_far_below_the_bound(ctx, hostile, dtype, e4m3, rows, context, heads, kv_heads, max_keys, options):
+    """Fewer chunks of keys than the CTAs that the host's bound calls for: some have nothing to do."""
+    from plm import cache as api
+
+    st = Setup(rows=rows, context=context, kv_heads=kv_heads, head_dim=128, page=16, dtype=dtype, e4m3=e4m3,
+               seed=len(rows) + heads)
+    st.poison_behind()
+    q = st.randn(st.total, heads, 128)
+    want, bound = st.expected(q, **options)
+    for seqs in _loose(st, max_keys):
+        assert within(api.attention(ctx, st.cache, seqs, q, **options), want, bound)
+    ctx.check()
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("rows,heads", [([1], 8), ([1, 2], 4), ([40], 4)])
+def test_one_graph_from_short_to_long_and_back(ctx, hostile, e4m3, rows, heads):
+    """A graph captured under a large bound serves every length below it."""
+    from plm import cache as api
+
+    longest = 2000
+    st = Setup(rows=rows, context=[longest] * len(rows), kv_heads=4, head_dim=128, page=16, dtype="bf16", e4m3=e4m3, seed=3)
+    q = st.randn(st.total, heads, 128)
+    seqs = _loose(st, 32768)[0]
+    api.attention(ctx, st.cache, seqs, q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = api.attention(ctx, st.cache, seqs, q)
+    for context in (0, 30, 100, 333, longest, 64, 3):
+        st.ctx_host = [max(0, context - 5 * s) for s in range(len(rows))]
+        st.seqs.context.copy_(torch.tensor(st.ctx_host, device="cuda"))
+        out.fill_(7.0)
+        graph.replay()
+        ctx.check()
+        want, bound = st.expected(q)
+        assert within(out, want, bound), context
+
+
+def test_c_entry_points_with_a_workspace_of_the_callers(ctx):
+    """plm.native's functions with descriptors of one's own: a workspace of NaN, and nothing written behind it."""
+    from plm import cache as api
+    from plm import native
+
+    st = Setup(rows=[1, 1], context=[60, 199], kv_heads=8, head_dim=128, page=16, dtype="bf16", e4m3=True, seed=2)
+    q, k, v = st.randn(2, 8, 128), st.randn(2, 8, 128), st.randn(2, 8, 128)
+    seqs = _loose(st, 32768)[0]
+    model = st.model()
+    model.append(st.starts, st.ctx_host, st.tables, k.double().cpu(), v.double().cpu())
+    row = 8 * 128
+    native.cache_append(ctx, native.CacheAppendDesc(dtype=native.PLM_BF16, rows=2, k=k.data_ptr(), v=v.data_ptr(), k_stride=row,
+                                                    v_stride=row, cache=st.cache.desc, seqs=seqs.desc))
+    _assert_pages(st.cache, model)
+    out = torch.zeros_like(q)
+    desc = native.CacheAttentionDesc(dtype=native.PLM_BF16, rows=2, q=q.data_ptr(), q_stride=row, out=out.data_ptr(),
+                                     out_stride=row, num_heads=8, cache=st.cache.desc, seqs=seqs.desc)
+    size = native.cache_attention_workspace(ctx, desc)
+    workspace = torch.full((size + 4096,), 0xFF, dtype=torch.uint8, device="cuda")
+    desc.workspace, desc.workspace_bytes = workspace.data_ptr(), size
+    native.cache_attention(ctx, desc)
+    ctx.check()
+    want, bound = st.expected(q)
+    assert within(out, want, bound)
+    assert (workspace[size:] == 0xFF).all()
+    assert torch.equal(_bits(out), _bits(api.attention(ctx, st.cache, seqs, q)))
