@@ -158,6 +158,7 @@ __device__ __forceinline__ TileKeys few_rows_keys(const CacheAttnArgs& a, const 
     t.sinks = min(a.sinks, t.lo);
   }
   t.count<kChunk>();
+  t.chunks = max(t.chunks, 1);  // rows that see no key have a chunk to themselves all the same, of zeros, and give zeros
   return t;
 }
 

@@ -6,7 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from tests.cache_reference import within
+from tests.cache_reference import UNREACHABLE, within
 from tests.test_cache_ops import PAGES, Setup, _assert_pages, _bits
 
 pytestmark = pytest.mark.gpu
@@ -112,3 +112,38 @@ def test_c_entry_points_with_a_workspace_of_the_callers(ctx):
     assert within(out, want, bound)
     assert (workspace[size:] == 0xFF).all()
     assert torch.equal(_bits(out), _bits(api.attention(ctx, st.cache, seqs, q)))
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("rows,context,depth", [
+    ([1], [15], 5), ([1], [63], 16), ([4], [12], 1 << 30), ([16], [0], 40), ([40], [8], 300), ([200], [56], 1 << 30),
+    ([1, 1, 1], [31, 20, 47], 100), ([3, 2], [13, 62], 70),
+    ([1] * 1100, [15] * 1100, 9),                      # more sequences than one even launch takes
+])
+def test_window_past_every_key_gives_zeros(ctx, e4m3, rows, context, depth):
+    """A window that lies behind all keys of a sequence, and no sinks: zeros, also where keys end with a chunk or a tile."""
+    from plm import cache as api
+
+    st = Setup(rows=rows, context=context, kv_heads=2, head_dim=128, page=16, dtype="bf16", e4m3=e4m3, seed=rows[0],
+               spare_rows=2)
+    q = st.randn(st.held, 2, 128)
+    out = torch.full_like(q, 7.0)
+    api.attention(ctx, st.cache, st.seqs, q, out=out, window=2, depth=_int32([depth] * st.held),
+                  own_start=_int32([UNREACHABLE] * st.held))
+    ctx.check()
+    assert (out[:st.total] == 0).all() and (out[st.total:] == 7.0).all()
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_window_past_the_keys_of_one_sequence(ctx, e4m3):
+    """Beside a sequence whose rows see nothing the others keep their results."""
+    from plm import cache as api
+
+    st = Setup(rows=[1, 1, 1], context=[300, 31, 100], kv_heads=2, head_dim=128, page=16, dtype="bf16", e4m3=e4m3, seed=1)
+    q = st.randn(3, 2, 128)
+    depth, own = _int32([0, 500, 0]), _int32([UNREACHABLE] * 3)
+    out = torch.full_like(q, 7.0)
+    api.attention(ctx, st.cache, st.seqs, q, out=out, window=64, depth=depth, own_start=own)
+    ctx.check()
+    want, bound = st.expected(q, window=64, depth=depth, own_start=own)
+    assert within(out, want, bound) and (out[1] == 0).all()
