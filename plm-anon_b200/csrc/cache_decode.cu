@@ -459,8 +459,9 @@ __global__ void __launch_bounds__(kThreads, E4M3 && NR == 1 ? 2 : 1) decode_atte
         p[nr][0] = transpose_8x8(pack2<M>(w[0], w[1]));
         p[nr][1] = transpose_8x8(pack2<M>(w[2], w[3]));
       }
-      // ---- values that are no numbers, where not every row sees every key
-      if (!full && r.n > 1) {
+      // ---- values that are no numbers, where not every row sees every key (a causal sequence's only row sees all that are
+      // loaded; under depth even that one may not)
+      if (!full && (r.n > 1 || a.depth != nullptr)) {
         constexpr int PER = 4 / ES;  // elements of a word
         bool any = false;
 #pragma unroll

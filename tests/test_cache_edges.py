@@ -147,3 +147,34 @@ def test_window_past_the_keys_of_one_sequence(ctx, e4m3):
     ctx.check()
     want, bound = st.expected(q, window=64, depth=depth, own_start=own)
     assert within(out, want, bound) and (out[1] == 0).all()
+
+
+@pytest.mark.parametrize("dtype,e4m3", PAGES)
+@pytest.mark.parametrize("context,depth,own", [(0, -1, UNREACHABLE), (50, -1, UNREACHABLE), (50, -9, 0), (200, -40, -3),
+                                               (15, -1, UNREACHABLE)])
+@pytest.mark.parametrize("rows", [[1], [1, 1, 1], [1, 2]])
+def test_a_single_row_may_hide_anything(ctx, dtype, e4m3, context, depth, own, rows):
+    """One row, which does not see all keys up to its own: what the hidden ones hold stays out of it."""
+    from plm import cache as api
+
+    st = Setup(rows=rows, context=[context] * len(rows), kv_heads=2, head_dim=128, page=16, dtype=dtype, e4m3=e4m3, seed=4)
+    first = context + depth + 1  # hidden, up to the own block or the row itself
+    last = context + (own if own <= 0 else 1)
+    for s in range(len(rows)):
+        for kv in range(max(first, 0), last):
+            p, slot = st.tables[s][kv // 16], kv % 16
+            for t in (st.cache.k, st.cache.v):
+                if e4m3:
+                    t.view(torch.uint8)[p, :, slot] = 0x7F
+                else:
+                    t[p, :, slot] = float("nan") if kv % 2 else float("inf")
+    q = st.randn(st.total, 4, 128)
+    depths, owns = _int32([depth] * st.total), _int32([own] * st.total)
+    out = api.attention(ctx, st.cache, st.seqs, q, depth=depths, own_start=owns)
+    ctx.check()
+    want, bound = st.expected(q, depth=depths, own_start=owns)
+    assert within(out[0], want[0], bound[0])  # of a sequence's second row the hidden tokens are its first row's
+    if context == 0:
+        assert (out[0] == 0).all()
+    if len(rows) == 3:
+        assert within(out, want, bound)
