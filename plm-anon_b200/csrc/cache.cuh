@@ -12,7 +12,8 @@ __device__ __forceinline__ SeqRange sequence_range(const CacheSeqs& s, int i, in
   const int lo = s.row_start[i], hi = s.row_start[i + 1];
   const int64_t context = s.context[i];
   SeqRange r = {lo, hi - lo, context};
-  if (lo < 0 || hi < lo || hi > s.rows || r.n > s.max_rows || context < 0 || context + r.n > s.max_tokens) {
+  // Of any context, 2^63 - 1 included: context + r.n could pass 64 bits.
+  if (lo < 0 || hi < lo || hi > s.rows || r.n > s.max_rows || context < 0 || context > s.max_tokens - r.n) {
     record_error(err, kErrBadIndex);
     r.n = 0;
   }

@@ -178,3 +178,28 @@ def test_a_single_row_may_hide_anything(ctx, dtype, e4m3, context, depth, own, r
         assert (out[0] == 0).all()
     if len(rows) == 3:
         assert within(out, want, bound)
+
+
+@pytest.mark.parametrize("rows", [1, 30])
+@pytest.mark.parametrize("context", [(1 << 63) - 1, (1 << 63) - 30, 1 << 62, (1 << 32) + 60, -(1 << 63)])
+def test_context_past_every_number(ctx, rows, context):
+    """A context whose sum with the rows passes 64 bits is one that the block table does not hold: skipped and recorded."""
+    from plm import cache as api
+    from plm.native import NativeError
+
+    st = Setup(rows=[rows] * 3, context=[50, 60, 70], kv_heads=2, head_dim=64, page=16, dtype="bf16", e4m3=True, seed=9)
+    q, k, v = st.randn(st.total, 2, 64), st.randn(st.total, 2, 64), st.randn(st.total, 2, 64)
+    good = api.attention(ctx, st.cache, st.seqs, q)
+    st.seqs.context[1] = context
+    out = torch.full_like(q, 7.0)
+    api.attention(ctx, st.cache, st.seqs, q, out=out)
+    with pytest.raises(NativeError, match="out of range"):
+        ctx.check()
+    assert torch.equal(_bits(out[:rows]), _bits(good[:rows])) and torch.equal(_bits(out[2 * rows:]), _bits(good[2 * rows:]))
+    assert (out[rows:2 * rows] == 7.0).all()
+    before = st.cache.k.view(torch.uint8).clone()
+    api.append(ctx, st.cache, st.seqs, k, v)
+    with pytest.raises(NativeError, match="out of range"):
+        ctx.check()
+    changed = (st.cache.k.view(torch.uint8) != before).flatten(1).any(dim=1).nonzero().flatten().tolist()
+    assert changed and set(changed) <= set(st.tables[0]) | set(st.tables[2])
