@@ -297,9 +297,10 @@ typedef struct plm_sequences {
  * once, to the model dtype or to e4m3. In e4m3 pages the scale of a block and head is 2^e, e the smallest integer with
  * max|x| <= 448 * 2^e over the call's finite values of that block, at least -100. A block that holds earlier tokens of
  * its sequence keeps the larger of the new and the old scale, and those tokens' codes are brought to it; tokens behind
- * the appended ones in the block are no longer valid. Infinities become +-448 times the scale, NaN stays NaN. Rows that no
- * sequence holds, and pages and blocks that no row falls into, are left as they were. No two sequences of a call may
- * append into one page. */
+ * the appended ones in the block are no longer valid. Infinities become +-448 times the scale, NaN stays NaN. A row whose
+ * position cos_sin does not have is recorded as an index out of range and left out: its query, key and value are not
+ * written, and it has no say in a scale. Rows that no sequence holds, and pages and blocks that no row falls into, are
+ * left as they were. No two sequences of a call may append into one page. */
 typedef struct plm_cache_append_desc {
   int32_t dtype;           /* enum plm_dtype: q, k, v, q_out, cos_sin and 16-bit pages */
   int32_t rows;            /* rows of the buffers */

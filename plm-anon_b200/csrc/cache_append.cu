@@ -62,16 +62,21 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
   *reinterpret_cast<uint4*>(p) = v;
 }
 
-// Rotates (a, b) = elements [8 chunk, + 8) of both halves of a head at the row's position.
+// Whether the table has the row's position, *pos (0 where it has not: that is recorded, and the row is left out).
+__device__ __forceinline__ bool row_position(const AppendArgs& a, int row, int64_t logical, int64_t* pos) {
+  *pos = 0;
+  if (a.cos_sin == nullptr) return true;
+  const int64_t given = a.positions != nullptr ? a.positions[row] : logical;
+  const bool there = given >= 0 && given < a.max_pos;
+  if (there) *pos = given;
+  else record_error(a.err, kErrBadIndex);
+  return there;
+}
+
+// Rotates (a, b) = elements [8 chunk, + 8) of both halves of a head at position `pos`.
 template <int HD, typename T>
-__device__ __forceinline__ void rotate(const AppendArgs& a, int row, int64_t logical, int chunk, float (&lo)[8],
-                                       float (&hi)[8]) {
+__device__ __forceinline__ void rotate(const AppendArgs& a, int64_t pos, int chunk, float (&lo)[8], float (&hi)[8]) {
   if (a.cos_sin == nullptr) return;
-  int64_t pos = a.positions != nullptr ? a.positions[row] : logical;
-  if (pos < 0 || pos >= a.max_pos) {
-    record_error(a.err, kErrBadIndex);
-    pos = 0;
-  }
   const T* cs = static_cast<const T*>(a.cos_sin) + size_t(pos) * HD + chunk * 8;
   float c[8], s[8];
   load8<T>(cs, c);
@@ -98,7 +103,9 @@ __device__ __forceinline__ void append_16bit(const AppendArgs& a, int row, int s
     const T* src = static_cast<const T*>(a.q) + row * a.q_stride + slot * HD + chunk * 8;
     load8<T>(src, lo);
     load8<T>(src + HD / 2, hi);
-    rotate<HD, T>(a, row, logical, chunk, lo, hi);
+    int64_t pos;
+    if (!row_position(a, row, logical, &pos)) return;
+    rotate<HD, T>(a, pos, chunk, lo, hi);
     T* dst = static_cast<T*>(a.q_out) + row * a.q_out_stride + slot * HD + chunk * 8;
     store8<T>(dst, lo);
     store8<T>(dst + HD / 2, hi);
@@ -115,7 +122,9 @@ __device__ __forceinline__ void append_16bit(const AppendArgs& a, int row, int s
            ((size_t(page) * a.c.kv_heads + head) * a.c.page_size + size_t(logical & (a.c.page_size - 1))) * HD + chunk * 8;
   load8<T>(src, lo);
   load8<T>(src + HD / 2, hi);
-  if (key) rotate<HD, T>(a, row, logical, chunk, lo, hi);
+  int64_t pos;
+  if (!row_position(a, row, logical, &pos)) return;
+  if (key) rotate<HD, T>(a, pos, chunk, lo, hi);
   store8<T>(dst, lo);
   store8<T>(dst + HD / 2, hi);
 }
@@ -220,12 +229,18 @@ __global__ void __launch_bounds__(2 * kAppendThreads) append_e4m3_kernel(const A
     load8<T>(src + row * stride + HD / 2, hi[p]);
   }
   const int page = physical_page(a.s, a.c, seq, first >> a.c.page_shift, a.err);
-  float amax = 0.f;
+  float amax = -1.f;  // of the tokens that have a position; below 0: there is none
+  uint32_t there = 0;  // those of this thread, by pass
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
     const int token = tid / CH + p * TOK;
     if (token < begin || token >= end) continue;
-    if (key) rotate<HD, T>(a, int(r.start + first + token - r.context), first + token, chunk, lo[p], hi[p]);
+    int64_t pos;
+    const bool counts = row_position(a, int(r.start + first + token - r.context), first + token, &pos);
+    if (key) rotate<HD, T>(a, pos, chunk, lo[p], hi[p]);
+    if (!counts) continue;
+    there |= 1u << p;
+    amax = fmaxf(amax, 0.f);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float x = fabsf(lo[p][e]), y = fabsf(hi[p][e]);
@@ -245,6 +260,7 @@ __global__ void __launch_bounds__(2 * kAppendThreads) append_e4m3_kernel(const A
   __syncthreads();  // also: every thread has read the old scale
 #pragma unroll
   for (int w = 0; w < kAppendThreads / 32; ++w) amax = fmaxf(amax, warp_amax[(key ? 0 : kAppendThreads / 32) + w]);
+  if (amax < 0.f) return;  // nothing to append: the block stays as it is
   const float now = fmaxf(exp2_int(scale_exponent(amax)), old);
   const float inverse = 1.f / now;
   if (tid == 0) *scale = now;
@@ -264,6 +280,8 @@ __global__ void __launch_bounds__(2 * kAppendThreads) append_e4m3_kernel(const A
         hi[p][e] = code_f32(e < 4 ? was[1].x : was[1].y, e & 3);
       }
       factor = old * inverse;
+    } else if (!(there >> p & 1)) {
+      continue;
     }
     uint32_t out[4];
 #pragma unroll

@@ -203,3 +203,62 @@ def test_context_past_every_number(ctx, rows, context):
         ctx.check()
     changed = (st.cache.k.view(torch.uint8) != before).flatten(1).any(dim=1).nonzero().flatten().tolist()
     assert changed and set(changed) <= set(st.tables[0]) | set(st.tables[2])
+
+
+@pytest.mark.parametrize("dtype,e4m3", PAGES)
+@pytest.mark.parametrize("head_dim,block", [(64, 16), (128, 16), (64, 64), (128, 64)])
+def test_append_skips_rows_without_a_position(ctx, dtype, e4m3, head_dim, block):
+    """A row whose position lies outside the table is recorded and left out: query, key, value, and its say in a scale."""
+    from plm import cache as api
+    from plm.native import NativeError
+    from plm.model import rope_cache
+
+    st = Setup(rows=[30, 70], context=[40, 3], kv_heads=2, head_dim=head_dim, page=64, dtype=dtype, e4m3=e4m3, block=block, seed=4)
+    cos_sin = rope_cache(head_dim, 50, 10000.0, st.dtype).cuda()
+    q, k, v = st.randn(100, 4, head_dim), st.randn(100, 2, head_dim), st.randn(100, 2, head_dim)
+    positions = torch.randint(0, 50, (100,), generator=st.g, device="cuda").to(torch.int32)
+    bad = [0, 7, 29, 33, 99] + list(range(43, 63))  # the last ones all of a block of 16 tokens (logical 16 .. 31)
+    for i, r in enumerate(bad):
+        positions[r] = (-1, 50, 1 << 30, -(1 << 31))[i % 4]
+        k[r] *= 100.0
+        v[r] *= 100.0
+    whole = [t.clone() for t in (st.cache.k.view(torch.uint8), st.cache.v.view(torch.uint8))]
+    scales = None if not e4m3 else [st.cache.k_scale.clone(), st.cache.v_scale.clone()]
+    q_out = torch.full_like(q, 7.0)
+    api.append(ctx, st.cache, st.seqs, k, v, q=q, q_out=q_out, cos_sin=cos_sin, positions=positions)
+    with pytest.raises(NativeError, match="out of range"):
+        ctx.check()
+    got = api.PagedCache(st.cache.k.clone(), st.cache.v.clone(), *([st.cache.k_scale.clone(), st.cache.v_scale.clone()] if e4m3 else []))
+    assert (q_out[bad] == 7.0).all()
+    rest = [r for r in range(100) if r not in bad]
+    assert not (q_out[rest] == 7.0).all(dim=-1).any()
+    places = {}
+    for s in range(2):
+        for r in range(st.starts[s], st.starts[s + 1]):
+            logical = st.ctx_host[s] + r - st.starts[s]
+            places[r] = (st.tables[s][logical // 64], logical % 64)
+    for plane, was in ((got.k, whole[0]), (got.v, whole[1])):
+        plane, was = plane.view(torch.uint8), was.view(torch.uint8)
+        for r in bad:
+            p, slot = places[r]
+            assert torch.equal(plane[p, :, slot], was[p, :, slot])
+    # the others as if the bad rows were as small as can be: zeros at a good position
+    st.cache.k.view(torch.uint8).copy_(whole[0])
+    st.cache.v.view(torch.uint8).copy_(whole[1])
+    if e4m3:
+        st.cache.k_scale.copy_(scales[0])
+        st.cache.v_scale.copy_(scales[1])
+    for r in bad:
+        positions[r], k[r], v[r] = 0, 0.0, 0.0
+    api.append(ctx, st.cache, st.seqs, k, v, q=q, q_out=q_out, cos_sin=cos_sin, positions=positions)
+    ctx.check()
+    for r in rest:
+        p, slot = places[r]
+        for a, b in ((got.k, st.cache.k), (got.v, st.cache.v)):
+            assert torch.equal(a.view(torch.uint8)[p, :, slot], b.view(torch.uint8)[p, :, slot])
+        if e4m3:
+            for a, b in ((got.k_scale, st.cache.k_scale), (got.v_scale, st.cache.v_scale)):
+                assert torch.equal(a[p, :, slot // block], b[p, :, slot // block])
+    if e4m3 and block == 16:  # no row of it: the block is as it was
+        p = st.tables[1][0]
+        assert torch.equal(got.k_scale[p, :, 1], scales[0][p, :, 1]) and torch.equal(got.v_scale[p, :, 1], scales[1][p, :, 1])
