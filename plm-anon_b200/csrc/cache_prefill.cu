@@ -46,7 +46,7 @@ constexpr int kRoleThreads = 128;
 constexpr int kPrefillThreads = 3 * kRoleThreads + 64;
 constexpr int kScaleSlots = 4;
 constexpr uint32_t kTmemColumns = 512;
-constexpr float kGuess = 4.f;  // log2 of how far the first weights may stay below 1
+constexpr float kGuess = -4.f;  // a row's maximum, in units of log2, before it has seen a key
 
 constexpr int kFetchBytes = 3328;
 
@@ -788,12 +788,13 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
         }
       };
       if constexpr (!E4M3) {
-        // One pass with the maximum as it is, 0 for a row that has seen no key yet; should it prove too small, or the
-        // guess too large, it is put right and the pass repeated.
+        // One pass with the maximum as it is, a guess for a row that has seen no key yet; should it prove too small, or the
+        // guess too large, it is put right and the pass repeated. So a row's largest weight is never below 1, and f16,
+        // whose smallest step is 2^-24, holds the others to 2^-25 of it.
         uint32_t p[kTile / 2];
         while (true) {
           const bool fresh = m == -INFINITY;
-          const float from = add - (fresh ? 0.f : m);
+          const float from = add - (fresh ? kGuess : m);
           const f32x2 scale2 = pair(by, by), from2 = pair(from, from);
           f32x2 sums[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
           float top = -INFINITY;
@@ -823,12 +824,12 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
             }
           }
           top = top == -INFINITY ? top : fmaf(top, by, add);
-          const bool again = fresh ? top > kLazy || (top < -kGuess && top > -INFINITY) : top > m + kLazy;
+          const bool again = top > (fresh ? kGuess : m) + kLazy || (fresh && top < kGuess && top > -INFINITY);
           if (!__any_sync(0xffffffffu, again)) {
             float lo, hi;
             unpair(add2(sums[0], sums[1]), lo, hi);
             l = fmaf(lo + hi, inv_v, l);
-            if (fresh && top > -INFINITY) m = 0.f;
+            if (fresh && top > -INFINITY) m = kGuess;
             break;
           }
           raise(top);

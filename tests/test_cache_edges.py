@@ -262,3 +262,25 @@ def test_append_skips_rows_without_a_position(ctx, dtype, e4m3, head_dim, block)
     if e4m3 and block == 16:  # no row of it: the block is as it was
         p = st.tables[1][0]
         assert torch.equal(got.k_scale[p, :, 1], scales[0][p, :, 1]) and torch.equal(got.v_scale[p, :, 1], scales[1][p, :, 1])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("rows", [40, 200])
+def test_prefill_weights_far_below_the_largest(ctx, dtype, rows):
+    """A largest score below 0 and many more than 2^20 below it: their share of the sum is not rounded away."""
+    from plm import cache as api
+
+    context = 1024 - rows
+    st = Setup(rows=[rows], context=[context], kv_heads=1, head_dim=64, page=16, dtype=dtype, e4m3=False, seed=1)
+    for kv in range(context + rows):
+        p, slot = st.tables[0][kv // 16], kv % 16
+        large = kv % 128 == 0
+        st.cache.k[p, 0, slot] = 0.0
+        st.cache.k[p, 0, slot, 0] = -2.75 if large else -17.0  # 2^-3.97 and 2^-24.5
+        st.cache.v[p, 0, slot] = 0.0 if large else 512.0
+    q = torch.zeros(rows, 1, 64, dtype=st.dtype, device="cuda")
+    q[:, :, 0] = 1.0
+    out = api.attention(ctx, st.cache, st.seqs, q, scale=1.0)
+    ctx.check()
+    want, bound = st.expected(q, scale=1.0)
+    assert within(out, want, bound)
