@@ -11,6 +11,7 @@ namespace plm {
 
 constexpr int kUnreachable = 1 << 30;  // no key's index: block tables hold less than 2^30 tokens
 constexpr float kLazy = 15.f;          // log2 of how far a weight may pass 1 before its row's maximum is raised: f16 holds it
+constexpr float kUsual = 45.f;         // log2 of scales between whose keys weights of 2^-30 of the largest are floats
 constexpr float kLeastScale = 7.888609052210118e-31f;  // 2^-100: smaller value scales count as this
 
 // 2^x by the special-function unit (relative error 2^-22; -inf gives +0, NaN stays).
@@ -31,6 +32,20 @@ __device__ __forceinline__ float rcp(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// In e4m3 pages the scales s of two values may lie so far apart that the weight w = 2^(score + log2 s - m) of one is no
+// float, although its share w / s of the sum l is as large as the other one's: a block of zeros (s = 2^-100) beside values
+// of 10^11. That share, 2^(score - m), from x = score + log2 s - m and log2 s:
+__device__ __forceinline__ float small_share(float x, float log_v) {
+  constexpr float kLift = 50.f;
+  return ex2(x - log_v + kLift) * 8.881784197001252e-16f;  // 2^-50
+}
+// 2^x as a factor of partial results: of l by its root twice, as l 2^x may be a float where 2^x is none.
+struct Keep {
+  float root;
+  __device__ __forceinline__ explicit Keep(float x) : root(ex2(0.5f * x)) {}
+  __device__ __forceinline__ float o() const { return root * root; }
+  __device__ __forceinline__ float l(float l) const { return l * root * root; }
+};
 // Two floats rounded to the 16-bit type M, `lo` in the low half.
 template <typename M>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -191,7 +206,8 @@ __device__ __forceinline__ void join_row(const CacheAttnArgs& a, int count, Part
   for (int base = 0; base < count; base += 32) {
     float2 mine = make_float2(-INFINITY, 0.f);
     if (base + lane < count) mine = *reinterpret_cast<const float2*>(part(base + lane) + ml);
-    const float f = ex2(mine.x - from);
+    const Keep keep(mine.x - from);
+    const float f = keep.o();
     const int here = min(32, count - base);
 #pragma unroll 8
     for (int x = 0; x < here; ++x) {
@@ -200,10 +216,10 @@ __device__ __forceinline__ void join_row(const CacheAttnArgs& a, int count, Part
       if constexpr (N == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
       else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
       const float w = __shfl_sync(0xffffffffu, f, x);
-      total = fmaf(w, __shfl_sync(0xffffffffu, mine.y, x), total);
 #pragma unroll
       for (int e = 0; e < N; ++e) sum[e] = fmaf(w, v[e], sum[e]);
     }
+    total += warp_sum(keep.l(mine.y));
   }
   store_row<T>(a, row0, i, head, HD, lane * N, sum, total);
 }

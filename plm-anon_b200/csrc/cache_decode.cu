@@ -32,7 +32,8 @@
 // e4m3 pages: codes become f16 exactly, and their scales never touch a 16-bit number. A key's scale multiplies its
 // scores. A value's scale s enters through w = 2^(score + log2 s - m): O += w code and l += w / s, out = O / l, so that
 // m follows the largest term of the sum, w <= 2^15 whatever the scales are, and rounding w to f16 (2^-11) is relative to
-// that term. Queries in bf16 become f16 exactly but for elements below 2^-30 of their row's largest (query_exponent).
+// that term. A weight that is too small for a float still counts in l (small_share). Queries in bf16 become f16 exactly
+// but for elements below 2^-30 of their row's largest (query_exponent).
 // 16-bit pages: products in the model dtype, w rounded to it, as in round_attention_kernel.
 //
 // Masks. Keys that no row of the tile sees are not loaded (their places are zeroed, so stale slots, or pages that were
@@ -358,6 +359,7 @@ __global__ void __launch_bounds__(kThreads, E4M3 && NR == 1 ? 2 : 1) decode_atte
     int pages = -1;
     if (c_first + (kStages - 1) * kWarps < c_end) pages = pages_of(t.key<kChunk>(c_first + (kStages - 1) * kWarps));
 
+    bool apart = false;  // scales were met with which a weight may be too small for a float
     int stage = 0;
     for (int c = c_first; c < c_end; c += kWarps) {
       const int kv0 = t.key<kChunk>(c);
@@ -425,23 +427,42 @@ __global__ void __launch_bounds__(kThreads, E4M3 && NR == 1 ? 2 : 1) decode_atte
           raise |= x > m[nr][e & 1] + kLazy;
         }
       }
-      if (__any_sync(0xffffffffu, raise)) {
+      if (__any_sync(0xffffffffu, raise || (E4M3 && (apart || fabsf(log_v[0]) > kUsual || fabsf(log_v[1]) > kUsual)))) {
+        if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
-        for (int nr = 0; nr < NR; ++nr) {
+          for (int nr = 0; nr < NR; ++nr) {
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            float top = fmaxf(s[nr][x], s[nr][x + 2]);
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-            top = fmaxf(top, m[nr][x]);
-            const float keep = ex2(m[nr][x] - (top == -INFINITY ? 0.f : top));
-            m[nr][x] = top;
-            l[nr][x] *= keep;
+            for (int x = 0; x < 2; ++x) {
+              float top = fmaxf(s[nr][x], s[nr][x + 2]);
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+              top = fmaxf(top, m[nr][x]);
+              const Keep keep(m[nr][x] - (top == -INFINITY ? 0.f : top));
+              m[nr][x] = top;
+              l[nr][x] = keep.l(l[nr][x]);
 #pragma unroll
-            for (int y = 0; y < KS; ++y) {
-              o[y][nr][x] *= keep;
-              o[y][nr][x + 2] *= keep;
+              for (int y = 0; y < KS; ++y) {
+                o[y][nr][x] *= keep.o();
+                o[y][nr][x + 2] *= keep.o();
+              }
+            }
+          }
+        }
+        if constexpr (E4M3) {
+#pragma unroll
+          for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) apart |= s[nr][e] > -INFINITY && fabsf(log_v[e >> 1]) > kUsual;
+          apart = __any_sync(0xffffffffu, apart);
+          if (apart) {
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float x = s[nr][e] - (m[nr][e & 1] == -INFINITY ? 0.f : m[nr][e & 1]);
+                if (ex2(x) == 0.f) l[nr][e & 1] += small_share(x, log_v[e >> 1]);
+              }
             }
           }
         }
@@ -560,13 +581,14 @@ __global__ void __launch_bounds__(kThreads, E4M3 && NR == 1 ? 2 : 1) decode_atte
       float total = 0.f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float f = ex2(pm[w][row] - from);
+        const Keep keep(pm[w][row] - from);
+        const float f = keep.o();
         const float4 x = *reinterpret_cast<const float4*>(&po[w][row][d]);
         sum.x += f * x.x;
         sum.y += f * x.y;
         sum.z += f * x.z;
         sum.w += f * x.w;
-        total += f * pl[w][row];
+        total += keep.l(pl[w][row]);
       }
       if (complete) {
         const float x[4] = {sum.x, sum.y, sum.z, sum.w};

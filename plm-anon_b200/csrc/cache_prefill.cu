@@ -139,6 +139,12 @@ __device__ __forceinline__ void tmem_ld_16(uint32_t taddr, float (&v)[16]) {
       : "r"(taddr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld_8(uint32_t taddr, float (&v)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+               : "r"(taddr)
+               : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_proxy_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -769,9 +775,9 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
       // A row's maximum to `top` (in units of log2), O and l with it.
       auto raise = [&](float top) {
         top = fmaxf(top, m);
-        const float keep = ex2(m - (top == -INFINITY ? 0.f : top));
+        const Keep keep(m - (top == -INFINITY ? 0.f : top));
         m = top;
-        l *= keep;
+        l = keep.l(l);
         if (done == 0) return;
         ok = warp_wait(bars->pv_done + stream, (done - 1) & 1, a.err, kErrTimeoutDone);
         if (!ok) return;
@@ -783,7 +789,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
           tmem_wait_ld();
           uint32_t z[16];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) z[e] = __float_as_uint(y[e] * keep);
+          for (int e = 0; e < 16; ++e) z[e] = __float_as_uint(y[e] * keep.o());
           tmem_st_16cols(t_o + c, z);
         }
       };
@@ -858,7 +864,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
             work(c + 32, x1);
           }
         };
-        float top = -INFINITY;
+        float top = -INFINITY, low = INFINITY;
         if (one) {
           each([&](int, const float(&x)[32]) {
             float tops[4] = {top, -INFINITY, -INFINITY, -INFINITY};
@@ -872,13 +878,20 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
         } else {
           each([&](int c, const float(&x)[32]) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) top = fmaxf(top, fmaf(x[e] * by, scales.k[c + e], scales.log_v[c + e]));
+            for (int e = 0; e < 32; ++e) {
+              const float y = fmaf(x[e] * by, scales.k[c + e], scales.log_v[c + e]);
+              top = fmaxf(top, y);
+              low = fminf(low, y == -INFINITY ? low : y);  // of the keys that the row sees
+            }
           });
         }
         if (__any_sync(0xffffffffu, top > m + kLazy)) raise(top);
         if (!ok) break;
         const float from = m == -INFINITY ? 0.f : m;
-        if (one) {
+        // With one scale it is the scores near the tile's largest that count, and their weights are floats unless that one
+        // itself stays this far below the row's maximum.
+        const bool apart = __any_sync(0xffffffffu, top > -INFINITY && top < m - 90.f);
+        if (one && !apart) {
           const f32x2 scale2 = pair(by, by), from2 = pair(add - from, add - from);
           f32x2 sums[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
           each([&](int c, const float(&x)[32]) {
@@ -898,6 +911,21 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
           unpair(add2(sums[0], sums[1]), lo, hi);
           l = fmaf(lo + hi, inv_v, l);
         } else {
+          const float by = fmaxf(q_scale, 1.17549435e-38f);  // the keys' scales come one by one
+          if (__any_sync(0xffffffffu, one || low < m - 125.f)) {
+#pragma unroll 1
+            for (int c = 0; c < kTile; c += 8) {  // little code: it is seldom run
+              float x[8];
+              tmem_ld_8(t_s + c, x);
+              tmem_wait_ld();
+              const uint32_t bits = full ? 0xffu : seen(c);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const float y = fmaf(x[e] * by, scales.k[c + e], scales.log_v[c + e]) - from;
+                if ((bits & (1u << e)) && ex2(y) == 0.f) l += small_share(y, scales.log_v[c + e]);
+              }
+            }
+          }
           each([&](int c, const float(&x)[32]) {
             uint32_t p[16];
 #pragma unroll
@@ -943,10 +971,11 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
       float keep0 = 1.f, keep1 = 0.f;
       if (!u.turns.two) {
         const float m1 = ml1[2 * row], top = fmaxf(m, m1), from = top == -INFINITY ? 0.f : top;
-        keep0 = ex2(m - from);
-        keep1 = ex2(m1 - from);
+        const Keep mine(m - from), other(m1 - from);
+        keep0 = mine.o();
+        keep1 = other.o();
         m = top;
-        l = l * keep0 + ml1[2 * row + 1] * keep1;
+        l = mine.l(l) + other.l(ml1[2 * row + 1]);
       }
       const bool theirs = keep1 > 0.f;  // stream 1 may not have had a tile: then its memory means nothing
       const float inverse = l == 0.f ? 0.f : 1.f / l;

@@ -284,3 +284,32 @@ def test_prefill_weights_far_below_the_largest(ctx, dtype, rows):
     ctx.check()
     want, bound = st.expected(q, scale=1.0)
     assert within(out, want, bound)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("rows", [1, 2, 60, 200])
+@pytest.mark.parametrize("exponent", [-10, 10, 30, 60, 90, 110])
+@pytest.mark.parametrize("context,block,apart", [(300, 16, False), (300, 2, False), (3000, 16, True)],
+                         ids=["blocks", "tokens", "halves"])
+def test_blocks_of_zeros_beside_large_values(ctx, dtype, rows, exponent, context, block, apart):
+    """Keys whose values are all zero, in blocks of the smallest scale, keep their share of the softmax's sum whatever the
+    other blocks' scales are: mixed with them, or the older half of a long context (parts of their own)."""
+    from plm import cache as api
+
+    if dtype == "f16" and exponent > 6:
+        exponent = 6  # the output has to hold the result
+    st = Setup(rows=[rows], context=[context], kv_heads=2, head_dim=128, page=16, dtype=dtype, e4m3=True, block=block,
+               seed=rows)
+    st.cache.k_scale.fill_(2.0 ** -7)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    zero = torch.rand(st.cache.v_scale.shape, generator=g, device="cuda") < 0.5
+    if apart:
+        zero[:] = False
+        zero[st.tables[0][:context // 32]] = True
+    st.cache.v_scale.copy_(torch.where(zero, 2.0 ** -100, 2.0 ** exponent))
+    st.cache.v.view(torch.uint8).masked_fill_(zero.repeat_interleave(block, dim=2)[..., None], 0)
+    q = st.randn(rows, 4, 128, scale=2.0)
+    out = api.attention(ctx, st.cache, st.seqs, q)
+    ctx.check()
+    want, bound = st.expected(q)
+    assert within(out, want, bound)
