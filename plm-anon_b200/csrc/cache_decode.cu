@@ -1,13 +1,13 @@
 // Attention over a paged cache for sequences of few rows (at most 16 packed rows: rows times query heads per kv head).
 // Every key and value is read once, 2 d bytes of e4m3 codes or 4 d of 16-bit numbers.
 //
-// What bounds it: with e4m3 pages the instructions that bring 16 keys through a warp, 427 (75 of them turn codes into
-// f16), two a clock on an SM whose schedulers are busy half of the time with 16 warps; with 16-bit pages (350) they are
+// What bounds it: with e4m3 pages the instructions that bring 16 keys through a warp, 434 (75 of them turn codes into
+// f16), two a clock on an SM whose schedulers are busy half of the time with 16 warps; with 16-bit pages (355) they are
 // busy a quarter of the time with 8 warps, 12 gain 1.5 %, and start, tail and join are what is left around the bytes.
-// Measured, head_dim 128, both launches: one token at 32768 e4m3 keys, 16
-// kv heads, 34.9 us (3.85 TB/s); one token of each of 61 sequences, 2 to 8191 e4m3 keys, 32 heads over 8, 121 us
-// (4.1 TB/s); of 8 sequences behind windows of 4096 16-bit keys, 32 heads over 8, 29.5 us (4.55 TB/s). One token at 1024
-// keys takes 9.8 us, all latency: few chunks to a warp, and join_kernel is a second launch.
+// Measured, head_dim 128, both launches: one token at 32768 e4m3 keys, 16 kv heads, 35.1 us (3.83 TB/s); one token of each
+// of 61 sequences, 2 to 8191 e4m3 keys, 32 heads over 8, 122 us (4.1 TB/s); of 8 sequences behind windows of 4096 16-bit
+// keys, 32 heads over 8, 29.9 us (4.5 TB/s). One token at 1024 keys takes 10 us, all latency: few chunks to a warp, and
+// join_kernel is a second launch.
 //
 // All chunks of 16 keys of all (sequence, kv head) tiles form one list, and the workers, the CTAs that fit on the GPU at
 // once, get equal shares of it, so uneven lengths and few heads keep every SM busy. The host sizes the grid by its bound on
@@ -630,7 +630,10 @@ bool one_row_tile(const CacheAttnArgs& a) { return int64_t(a.s.max_rows) * a.gro
 
 // Workers of an even launch: the CTAs that are resident at once, or fewer where each would get less than two chunks a
 // warp. Where that takes little away, as many to every tile: tiles of one length then begin with a worker, which has one
-// tile to fetch queries for and to join (8 windows of 4096 keys, 64 tiles on 148 SMs: 128 workers 29.5 us, 148 workers 32.0).
+// tile to fetch queries for and to join. That gains 6 to 9 % with sequences of one length and loses 2 to 8 % with ragged
+// ones, whose lengths the host does not know. 32 heads over 8, as many to every tile against all resident CTAs: 8
+// windows of 4096 16-bit keys 29.5 us, 32.0; 8 sequences of 8191 e4m3 keys 35.4, 38.6 (16-bit 47.8, 50.6); 8 of 2000 to 8191
+// 30.1, 28.9 (35.4, 34.2); 16 of 2 to 8191 67.6, 66.2 (74.6, 73.2); 2 of 101 and 32761 55.6, 51.3 (57.2, 57.8).
 int decode_workers(const CacheAttnArgs& a, int kind, int64_t max_keys, int num_sms) {
   const int64_t keys = a.window > 0 ? std::min<int64_t>(max_keys, int64_t(a.window) + a.sinks + a.s.max_rows) : max_keys;
   const int64_t tiles = int64_t(a.s.n_seqs) * a.c.kv_heads, chunks = tiles * ((keys + kChunk - 1) / kChunk);

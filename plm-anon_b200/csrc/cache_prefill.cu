@@ -23,7 +23,7 @@
 // f16 on the same schedulers. The first tile is in softmax 7 thousand clocks after the CTA starts, the output takes 6, so
 // the tensor core is busy 30 % of a call. With one row tile the rings of two hold one key tile for each stream, whose next
 // one is fetched late: 4 us a key tile and CTA (16 heads, 56 rows: 17 us over 256 keys, 32 over 4152, 77 over 16440).
-// Measured: 2048 rows, 16 heads, over 6000 + 2048 e4m3 keys 227 us (520 TFLOP/s, 32 % of a large bf16 product's rate);
+// Measured: 2048 rows, 16 heads, over 6000 + 2048 e4m3 keys 229 us (517 TFLOP/s, 31 % of a large bf16 product's rate);
 // 8191 rows, 16 heads over 4, window 1024, 139 us (465 TFLOP/s of visible pairs).
 //
 // Softmax: base 2, lazy maximum (O is rescaled only when a score passes m by more than 2^15), scales of e4m3 pages kept
@@ -1078,7 +1078,9 @@ int64_t prefill_units(const CacheAttnArgs& a) {
   return std::min<int64_t>(int64_t(a.s.rows) * a.group / kUnit + a.s.n_seqs, per_seq * a.s.n_seqs) * a.c.kv_heads;
 }
 
-// CTAs that share a unit's keys: as many as there are SMs for, with at least two key tiles each.
+// CTAs that share a unit's keys: as many as there are SMs for, with at least two key tiles each. It is one number for the
+// call: beside a prompt of many units a single token's keys are one CTA's for each kv head, however many they are (2048 rows
+// of 32 heads over 8, and one token at 32768 keys: e4m3 pages 84 us, 25 us, in one call 902; 16-bit 59, 32, 1470).
 int prefill_splits(const CacheAttnArgs& a, int64_t max_keys, int num_sms) {
   const int64_t keys = a.window > 0 ? std::min<int64_t>(max_keys, int64_t(a.window) + a.sinks + kUnit) : max_keys;
   const int64_t tiles = (keys + kTile - 1) / kTile;

@@ -43,7 +43,8 @@ def hostile(request, monkeypatch):
 @pytest.mark.parametrize("dtype,e4m3", PAGES)
 @pytest.mark.parametrize("rows,context,heads,kv_heads,max_keys,options", [
     ([1], [99], 16, 16, 8192, {}), ([1], [199], 32, 8, 32768, {}), ([1], [16], 1, 1, 8192, {}),
-    ([1], [299], 2, 1, 32768, {}), ([1] * 4, [49] * 4, 8, 8, 32768, {}), ([1] * 8, [17, 300, 45, 0, 80, 16, 15, 130], 2, 2, 8192, {}),
+    ([1], [299], 2, 1, 32768, {}), ([1] * 4, [49] * 4, 8, 8, 32768, {}),
+    ([1] * 8, [17, 300, 45, 0, 80, 16, 15, 130], 2, 2, 8192, {}),
     ([2] * 3, [250, 17, 60], 16, 2, 8192, {}),                             # 16 packed rows: the wider tile
     ([0] * 31 + [1] + [0] * 32, [511] * 64, 8, 8, 512, {}),                # slots of which one holds a row
     ([1] * 2, [120, 40], 8, 8, 32768, dict(window=4096, sinks=4)),         # contexts short of the window
@@ -213,7 +214,8 @@ def test_append_skips_rows_without_a_position(ctx, dtype, e4m3, head_dim, block)
     from plm.native import NativeError
     from plm.model import rope_cache
 
-    st = Setup(rows=[30, 70], context=[40, 3], kv_heads=2, head_dim=head_dim, page=64, dtype=dtype, e4m3=e4m3, block=block, seed=4)
+    st = Setup(rows=[30, 70], context=[40, 3], kv_heads=2, head_dim=head_dim, page=64, dtype=dtype, e4m3=e4m3, block=block,
+               seed=4)
     cos_sin = rope_cache(head_dim, 50, 10000.0, st.dtype).cuda()
     q, k, v = st.randn(100, 4, head_dim), st.randn(100, 2, head_dim), st.randn(100, 2, head_dim)
     positions = torch.randint(0, 50, (100,), generator=st.g, device="cuda").to(torch.int32)
@@ -228,7 +230,7 @@ def test_append_skips_rows_without_a_position(ctx, dtype, e4m3, head_dim, block)
     api.append(ctx, st.cache, st.seqs, k, v, q=q, q_out=q_out, cos_sin=cos_sin, positions=positions)
     with pytest.raises(NativeError, match="out of range"):
         ctx.check()
-    got = api.PagedCache(st.cache.k.clone(), st.cache.v.clone(), *([st.cache.k_scale.clone(), st.cache.v_scale.clone()] if e4m3 else []))
+    got = api.PagedCache(*(t.clone() for t in (st.cache.k, st.cache.v, st.cache.k_scale, st.cache.v_scale) if t is not None))
     assert (q_out[bad] == 7.0).all()
     rest = [r for r in range(100) if r not in bad]
     assert not (q_out[rest] == 7.0).all(dim=-1).any()
