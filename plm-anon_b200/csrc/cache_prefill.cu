@@ -23,7 +23,7 @@
 // f16 on the same schedulers. The first tile is in softmax 7 thousand clocks after the CTA starts, the output takes 6, so
 // the tensor core is busy 30 % of a call. With one row tile the rings of two hold one key tile for each stream, whose next
 // one is fetched late: 4 us a key tile and CTA (16 heads, 56 rows: 17 us over 256 keys, 32 over 4152, 77 over 16440).
-// Measured: 2048 rows, 16 heads, over 6000 + 2048 e4m3 keys 229 us (517 TFLOP/s, 31 % of a large bf16 product's rate);
+// Measured: 2048 rows, 16 heads, over 6000 + 2048 e4m3 keys 231 us (512 TFLOP/s, 31 % of a large bf16 product's rate);
 // 8191 rows, 16 heads over 4, window 1024, 139 us (465 TFLOP/s of visible pairs).
 //
 // Softmax: base 2, lazy maximum (O is rescaled only when a score passes m by more than 2^15), scales of e4m3 pages kept
@@ -66,7 +66,7 @@ struct PrefillSmem {
 struct PrefillBarriers {
   uint64_t q_ready, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], pv_done[2],
       scales_full[kScaleSlots];
-  int one[kScaleSlots];  // whether the tile has one scale
+  int one[kScaleSlots];  // 0: the tile has more than one scale; otherwise 1 + spread of its values'
   uint32_t tmem;
   int issuing;  // held by the stream that issues products
   int odd;  // a value that is no number was met in a masked tile
@@ -290,7 +290,10 @@ __device__ __forceinline__ void drop_non_finite(uint4& x) {
 
 // What softmax needs to know of a tile of e4m3 keys. Normally the scales of a tile are powers of two within 2^15 of
 // each other, and the codes are brought to the largest one's on the way into shared memory, exactly: then the tile has
-// one scale. Otherwise they stay as they are, and softmax applies the scales key by key.
+// one scale. Otherwise they stay as they are, and softmax applies the scales key by key. A weight that goes by the tile's
+// scale of values may lie above its key's own term by what the scales lie apart, 2^spread. Softmax keeps m so far below the
+// largest weight, so that f16, whose smallest step is 2^-24, holds every term to 2^-25 of the largest term of the sum; the
+// lazy maximum has that much less room (2048 rows over 8048 keys, scales within 1, 2^6, 2^10, 2^14 of each other: SPREADS).
 struct TileScales {
   float k[kTile], log_v[kTile], inv_v[kTile];  // by key; where `one`, the first of each is the tile's
 };
@@ -317,16 +320,18 @@ __device__ __forceinline__ void note_scales(FetchRows* rows, int which, bool liv
     rows->odd[which][tid >> 5] = odd ? 1 : 0;
   }
 }
-// Whether the tile has one scale, after a barrier; *top is the largest, *relative the share of it that `scale` is.
+// Whether the tile has one scale, after a barrier; *top is the largest, 2^*spread of the smallest, *relative the share of it
+// that `scale` is.
 __device__ __forceinline__ bool one_scale(const FetchRows* rows, int which, bool live, float scale, float* relative,
-                                          float* top) {
+                                          float* top, int* spread) {
   const float* low = rows->low[which];
   const float* high = rows->high[which];
   const int* odd = rows->odd[which];
   *top = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3]));
-  const bool one = (odd[0] | odd[1] | odd[2] | odd[3]) == 0 && *top > 0.f &&
-                   fminf(fminf(low[0], low[1]), fminf(low[2], low[3])) * 32768.f >= *top;
-  // the quotient of two powers of two
+  const float least = fminf(fminf(low[0], low[1]), fminf(low[2], low[3]));
+  const bool one = (odd[0] | odd[1] | odd[2] | odd[3]) == 0 && *top > 0.f && least * 32768.f >= *top;
+  // quotients of powers of two
+  *spread = int(__float_as_uint(*top) - __float_as_uint(least)) >> 23;
   *relative = one && live ? __uint_as_float(__float_as_uint(scale) - __float_as_uint(*top) + 0x3f800000u) : 1.f;
   return one;
 }
@@ -459,8 +464,9 @@ __device__ __forceinline__ void fetch_tiles(const CacheAttnArgs& a, const Unit& 
       note_scales(share, 1, live, vs);
       named_barrier_sync(NAMED, kRoleThreads);
       float k_relative, v_relative, k_top, v_top;
-      const bool k_one = one_scale(share, 0, live, ks, &k_relative, &k_top);
-      const bool v_one = one_scale(share, 1, live, vs, &v_relative, &v_top);
+      int k_spread, v_spread;
+      const bool k_one = one_scale(share, 0, live, ks, &k_relative, &k_top, &k_spread);
+      const bool v_one = one_scale(share, 1, live, vs, &v_relative, &v_top, &v_spread);
       share->k_relative[n & 1][tid] = k_relative;
       share->v_relative[n & 1][tid] = v_relative;
       mine = next;
@@ -476,7 +482,7 @@ __device__ __forceinline__ void fetch_tiles(const CacheAttnArgs& a, const Unit& 
         scales.k[tid] = k_one ? k_top : ks;
         scales.log_v[tid] = lg2(v);
         scales.inv_v[tid] = rcp(v);
-        if (tid == 0) bars->one[slot] = k_one && v_one ? 1 : 0;
+        if (tid == 0) bars->one[slot] = k_one && v_one ? 1 + v_spread : 0;
         named_barrier_sync(NAMED, kRoleThreads);  // and every key's share of the scale is there
         if (lane == 0) mbar_arrive(bars->scales_full + slot);
       }
@@ -885,7 +891,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) prefill_attention_kernel(c
             }
           });
         }
-        if (__any_sync(0xffffffffu, top > m + kLazy)) raise(top);
+        if (__any_sync(0xffffffffu, top > m + kLazy)) raise(one ? top - float(bars->one[slot] - 1) : top);
         if (!ok) break;
         const float from = m == -INFINITY ? 0.f : m;
         // With one scale it is the scores near the tile's largest that count, and their weights are floats unless that one

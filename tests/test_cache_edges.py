@@ -315,3 +315,33 @@ def test_blocks_of_zeros_beside_large_values(ctx, dtype, rows, exponent, context
     ctx.check()
     want, bound = st.expected(q)
     assert within(out, want, bound)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("rows", [40, 200])
+@pytest.mark.parametrize("ratio", [0, 3, 8, 11, 15])
+def test_prefill_weights_beside_smaller_values(ctx, dtype, rows, ratio):
+    """Few keys with the largest scores by far and values of a scale 2^-ratio: weights are rounded relative to the largest
+    term, score and scale together, also where a tile's codes are brought to one scale."""
+    from plm import cache as api
+
+    context = 1024 - rows
+    st = Setup(rows=[rows], context=[context], kv_heads=1, head_dim=64, page=16, dtype=dtype, e4m3=True, seed=1)
+    st.cache.k_scale.fill_(0.125)
+    st.cache.v_scale.fill_(1.0)
+    for s in (st.cache.k, st.cache.v):
+        s.view(torch.uint8).zero_()
+    for kv in range(context + rows):
+        p, slot = st.tables[0][kv // 16], kv % 16
+        large = kv % 128 == 16
+        if large:
+            st.cache.v_scale[p] = 2.0 ** -ratio
+        st.cache.v[p, 0, slot, :32] = torch.full((32,), 0.0 if large else 120.0, device="cuda").to(torch.float8_e4m3fn)
+        if not large:
+            st.cache.k[p, 0, slot, :1] = torch.full((1,), -144.0, device="cuda").to(torch.float8_e4m3fn)
+    q = torch.zeros(rows, 1, 64, dtype=st.dtype, device="cuda")
+    q[:, :, 0] = 1.0  # scores of 0 and of -18, 2^-26
+    out = api.attention(ctx, st.cache, st.seqs, q, scale=1.0)
+    ctx.check()
+    want, bound = st.expected(q, scale=1.0)
+    assert within(out, want, bound)
