@@ -22,8 +22,8 @@
 // streams take. With e4m3 pages it is 7 thousand: softmax goes in two short loops, and the fetching warps bring codes to
 // f16 on the same schedulers. The first tile is in softmax 7 thousand clocks after the CTA starts, the output takes 6, so
 // the tensor core is busy 30 % of a call. With one row tile the rings of two hold one key tile for each stream, whose next
-// one is fetched late: 4 us a key tile and CTA (16 heads, 56 rows: 17 us over 256 keys, 32 over 4152, 77 over 16440).
-// Measured: 2048 rows, 16 heads, over 6000 + 2048 e4m3 keys 231 us (512 TFLOP/s, 31 % of a large bf16 product's rate);
+// one is fetched late: 4 us a key tile and CTA (16 heads, 56 rows: 17 us over 256 keys, 33 over 4152, 72 over 16440).
+// Measured: 2048 rows, 16 heads, over 6000 + 2048 e4m3 keys 236 us (501 TFLOP/s, 31 % of a large bf16 product's rate);
 // 8191 rows, 16 heads over 4, window 1024, 139 us (465 TFLOP/s of visible pairs).
 //
 // Softmax: base 2, lazy maximum (O is rescaled only when a score passes m by more than 2^15), scales of e4m3 pages kept
@@ -293,7 +293,8 @@ __device__ __forceinline__ void drop_non_finite(uint4& x) {
 // one scale. Otherwise they stay as they are, and softmax applies the scales key by key. A weight that goes by the tile's
 // scale of values may lie above its key's own term by what the scales lie apart, 2^spread. Softmax keeps m so far below the
 // largest weight, so that f16, whose smallest step is 2^-24, holds every term to 2^-25 of the largest term of the sum; the
-// lazy maximum has that much less room (2048 rows over 8048 keys, scales within 1, 2^6, 2^10, 2^14 of each other: SPREADS).
+// lazy maximum has that much less room (2048 rows over 8048 keys, scales within 1, 2^6 and 2^14: 234, 236 and 238 us; one
+// fixed reserve of 2^5, and key by key beyond it: 231, 255 and 361).
 struct TileScales {
   float k[kTile], log_v[kTile], inv_v[kTile];  // by key; where `one`, the first of each is the tile's
 };
