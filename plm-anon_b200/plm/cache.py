@@ -205,8 +205,9 @@ def append(ctx: native.Context, cache: PagedCache, seqs: Sequences, k: torch.Ten
 
     ``q`` [rows, heads, head_dim], ``k`` and ``v`` [rows, kv_heads, head_dim] may be slices of one projection's rows.
     Returns the rotated queries: ``q_out`` (``q`` itself is allowed), or a new tensor. Rows that no sequence holds are not
-    written, and a row whose position ``cos_sin`` does not have is recorded and left out, key and value too. e4m3 pages: the call sets the scales of the blocks it begins and raises those it continues, bringing
-    the tokens before its own to the new scale; tokens behind the appended ones in a block are no longer valid."""
+    written, and a row whose position ``cos_sin`` does not have is recorded and left out, key and value too. e4m3 pages:
+    the call sets the scales of the blocks it begins and raises those it continues, bringing the tokens before its own to
+    the new scale; tokens behind the appended ones in a block are no longer valid."""
     what = "cache.append"
     rows, hd = k.shape[0], cache.head_dim
     dtype = k.dtype
